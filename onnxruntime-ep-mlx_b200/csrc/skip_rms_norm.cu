@@ -1,0 +1,249 @@
+// Residual addition + RMS norm, with a 16-bit or fp8 e4m3 output (b200_skip_rms_norm).
+//
+//   s = x + residual;  y = s / sqrt(mean(s^2) + eps) * weight;  fp8: code = e4m3(y / scale),
+//   scale = max|y| / 448 over the row or over a group of channels
+//
+// Memory bound (about 8 flops per 7 to 8 bytes).  One CTA owns a row and keeps its s in registers
+// (ITEMS vectors of VEC channels per thread), so every input is read once and every output written
+// once; the sum of squares and a row's maximum cross the CTA through shared memory, and a group of
+// channels that lies inside a warp needs shuffles only.  All sums are fp32 and their order is fixed
+// by the row's width, so a row's result does not depend on the batch around it.
+#include <algorithm>
+
+#include "b200_common.cuh"
+#include "layer_kernels.h"
+
+namespace b200 {
+namespace {
+
+constexpr float kFp8Max = 448.0f;
+constexpr float kAmaxFloor = 1e-12f;  // an all-zero row or group still gets a scale above zero
+
+template <int VEC> struct Raw;
+template <> struct Raw<8> { using type = uint4; };
+template <> struct Raw<4> { using type = uint2; };
+template <> struct Raw<1> { using type = uint16_t; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const typename Raw<VEC>::type& raw, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = act<T>::to_f(*reinterpret_cast<const T*>(&raw));
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      const float2 f = mma_op<T>::unpack(w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ typename Raw<VEC>::type pack(const float (&v)[VEC]) {
+  typename Raw<VEC>::type raw;
+  if constexpr (VEC == 1) {
+    const T t = act<T>::from_f(v[0]);
+    raw = *reinterpret_cast<const uint16_t*>(&t);
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) w[i] = mma_op<T>::pack(v[2 * i], v[2 * i + 1]);
+  }
+  return raw;
+}
+
+// VEC e4m3 codes of v * inv, saturating, as VEC bytes at dst (aligned to VEC).
+template <int VEC>
+__device__ __forceinline__ void store_e4m3(uint8_t* dst, const float (&v)[VEC], float inv) {
+  if constexpr (VEC == 1) {
+    *dst = (uint8_t)__nv_cvt_float_to_fp8(v[0] * inv, __NV_SATFINITE, __NV_E4M3);
+  } else {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+      w[i] = lo | (hi << 16);
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
+  }
+}
+
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+template <typename T, int VEC, int ITEMS, bool FP8>
+__global__ void __launch_bounds__(1024) skip_rms_norm_kernel(const B200SkipRmsNormParams p) {
+  using R = typename Raw<VEC>::type;
+  __shared__ float warp_sum[32];
+  __shared__ int group_max[B200_SKIP_RMS_NORM_MAX_HIDDEN / B200_SKIP_RMS_NORM_MIN_GROUP];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+  const int64_t row = blockIdx.x;
+  const int n = p.hidden / VEC;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_row_stride;
+  const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_row_stride : nullptr;
+  const T* weight = static_cast<const T*>(p.weight);
+
+  R xr[ITEMS], rr[ITEMS], wr[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = tid + k * threads;
+    xr[k] = rr[k] = wr[k] = R{};
+    if (i < n) {
+      xr[k] = *reinterpret_cast<const R*>(x + i * VEC);
+      if (res) rr[k] = *reinterpret_cast<const R*>(res + i * VEC);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k)
+    if (tid + k * threads < n) wr[k] = __ldg(reinterpret_cast<const R*>(weight) + tid + k * threads);
+
+  float s[ITEMS][VEC], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    float r[VEC];
+    unpack<T, VEC>(xr[k], s[k]);
+    unpack<T, VEC>(rr[k], r);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      s[k][j] += r[j];
+      sum += s[k][j] * s[k][j];
+    }
+  }
+  if (p.residual_out) {
+    T* ro = static_cast<T*>(p.residual_out) + row * p.residual_out_row_stride;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+      if (tid + k * threads < n) *reinterpret_cast<R*>(ro + (tid + k * threads) * VEC) = pack<T, VEC>(s[k]);
+  }
+  const int groups = FP8 && p.group_size ? (p.hidden + p.group_size - 1) / p.group_size : 1;
+  if (FP8)
+    for (int i = tid; i < groups; i += threads) group_max[i] = 0;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) warp_sum[warp] = sum;
+  __syncthreads();
+  sum = lane < (threads >> 5) ? warp_sum[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float rstd = 1.0f / sqrtf(sum / (float)p.hidden + p.epsilon);
+
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    float w[VEC];
+    unpack<T, VEC>(wr[k], w);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[k][j] = s[k][j] * rstd * w[j];
+  }
+  if constexpr (!FP8) {
+    T* out = static_cast<T*>(p.out) + row * p.out_row_stride;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+      if (tid + k * threads < n) *reinterpret_cast<R*>(out + (tid + k * threads) * VEC) = pack<T, VEC>(s[k]);
+  } else {
+    uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.out_row_stride;
+    float* scales = p.scales + row * groups;
+    // lanes of one warp that share a group; a group wider than a warp is joined in shared memory
+    const int lanes = p.group_size ? min(32, p.group_size / VEC) : 32;
+    const bool in_warp = p.group_size != 0 && p.group_size <= 32 * VEC;
+    float amax[ITEMS], row_max = 0.f;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      float m = 0.f;
+      if (tid + k * threads < n) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(s[k][j]));
+      }
+      amax[k] = m;
+      row_max = max_nan(row_max, m);
+    }
+    if (!p.group_size) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) row_max = max_nan(row_max, __shfl_xor_sync(0xffffffffu, row_max, o));
+      // magnitudes order like their bit patterns, a NaN above all
+      if (lane == 0) atomicMax(&group_max[0], __float_as_int(row_max));
+      __syncthreads();
+      const float scale = max_nan(__int_as_float(group_max[0]), kAmaxFloor) / kFp8Max;
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) amax[k] = scale;
+      if (tid == 0) scales[0] = scale;
+    } else {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        for (int o = lanes >> 1; o; o >>= 1) amax[k] = max_nan(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], o));
+      if (!in_warp) {
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k)
+          if (lane == 0 && tid + k * threads < n)
+            atomicMax(&group_max[(tid + k * threads) * VEC / p.group_size], __float_as_int(amax[k]));
+        __syncthreads();
+      }
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        const int c = (tid + k * threads) * VEC;
+        if (c >= p.hidden) continue;
+        const int g = c / p.group_size;
+        if (!in_warp) amax[k] = __int_as_float(group_max[g]);
+        amax[k] = max_nan(amax[k], kAmaxFloor) / kFp8Max;
+        if (c % p.group_size == 0) scales[g] = amax[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+      if (tid + k * threads < n) store_e4m3<VEC>(out + (tid + k * threads) * VEC, s[k], 1.0f / amax[k]);
+  }
+}
+
+template <typename T, int VEC, int ITEMS>
+void launch_items(const B200SkipRmsNormParams& p, int threads, cudaStream_t stream) {
+  if (p.out_dtype == B200_DTYPE_FLOAT8E4M3FN)
+    skip_rms_norm_kernel<T, VEC, ITEMS, true><<<p.rows, threads, 0, stream>>>(p);
+  else
+    skip_rms_norm_kernel<T, VEC, ITEMS, false><<<p.rows, threads, 0, stream>>>(p);
+}
+
+template <typename T, int VEC>
+void launch_vec(const B200SkipRmsNormParams& p, cudaStream_t stream) {
+  const int n = p.hidden / VEC;
+  auto threads_for = [&](int items) { return std::min(1024, ((n + items - 1) / items + 31) / 32 * 32); };
+  if (n <= 1024) launch_items<T, VEC, 1>(p, threads_for(1), stream);
+  else if (n <= 2048) launch_items<T, VEC, 2>(p, threads_for(2), stream);
+  else if (n <= 4096) launch_items<T, VEC, 4>(p, threads_for(4), stream);
+  else if constexpr (VEC <= 4) {
+    if (n <= 8192) launch_items<T, VEC, 8>(p, threads_for(8), stream);
+    else if constexpr (VEC == 1) launch_items<T, VEC, 32>(p, threads_for(32), stream);
+  }
+}
+
+template <typename T>
+void launch_type(const B200SkipRmsNormParams& p, cudaStream_t stream) {
+  // widest vector that every row of every 16-bit tensor starts on and that divides the row
+  const int out16 = p.out_dtype == p.dtype;
+  uintptr_t mask = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.residual) |
+                   reinterpret_cast<uintptr_t>(p.weight) | reinterpret_cast<uintptr_t>(p.residual_out) |
+                   (uintptr_t)(p.x_row_stride * 2) | (uintptr_t)p.hidden * 2;
+  if (p.residual) mask |= (uintptr_t)(p.residual_row_stride * 2);
+  if (p.residual_out) mask |= (uintptr_t)(p.residual_out_row_stride * 2);
+  mask |= out16 ? reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_row_stride * 2)
+                : (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row_stride) * 2;
+  if (mask % 16 == 0) launch_vec<T, 8>(p, stream);
+  else if (mask % 8 == 0) launch_vec<T, 4>(p, stream);
+  else launch_vec<T, 1>(p, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_skip_rms_norm(const B200SkipRmsNormParams& p, int, cudaStream_t stream) {
+  if (p.dtype == B200_DTYPE_BFLOAT16) launch_type<__nv_bfloat16>(p, stream);
+  else launch_type<__half>(p, stream);
+  add_launches(1);
+  return cudaGetLastError();
+}
+
+}  // namespace b200

@@ -3,7 +3,8 @@
 Mirrors the reference package's helper surface (python/src/onnxruntime_ep_mlx/__init__.py:43-167):
 ``EP_NAME``, ``library_path()`` and ``register_execution_provider_library()``, plus direct
 operator entry points (``paged_attention``, ``kv_append``) over the C ABI in
-``include/b200_paged.h``.
+``include/b200_paged.h`` and the decoder-layer operators around them (``skip_rms_norm``,
+``rotary_append``, ``shared_prefix_attention``) over ``include/b200_layer.h``.
 """
 
 from __future__ import annotations
@@ -11,6 +12,7 @@ from __future__ import annotations
 import os
 
 from ._capi import LIB, B200Error, library_file
+from .layer import rotary_append, shared_prefix_attention, skip_rms_norm
 from .paged import kv_append, paged_attention
 
 EP_NAME = "B200ExecutionProvider"
@@ -24,6 +26,9 @@ __all__ = [
     "kernel_library_path",
     "paged_attention",
     "register_execution_provider_library",
+    "rotary_append",
+    "shared_prefix_attention",
+    "skip_rms_norm",
 ]
 
 

@@ -1,5 +1,5 @@
-"""ctypes binding of ``include/b200_paged.h``, ``include/b200_ep.h`` and ``include/b200_shard.h``
-(the library's C ABI).
+"""ctypes binding of ``include/b200_paged.h``, ``include/b200_ep.h``, ``include/b200_shard.h`` and
+``include/b200_layer.h`` (the library's C ABI).
 
 The library is loaded from this package folder.  A missing or stale library raises at import
 time: there is no CPU fallback for the claimed path.
@@ -172,6 +172,46 @@ class ShardGatherParams(ctypes.Structure):
                 ("outputs", _vp * SHARD_MAX_RANKS), ("flags", _vp * SHARD_MAX_RANKS), ("state", _vp),
                 ("status", _vp), ("num_sms", _i32)]
 
+
+ROTARY_APPEND_SCAN_TOKENS = 8192
+
+
+class SkipRmsNormParams(ctypes.Structure):
+    """Mirror of ``B200SkipRmsNormParams`` (include/b200_layer.h)."""
+
+    _fields_ = [("rows", _i32), ("hidden", _i32), ("dtype", _i32), ("out_dtype", _i32), ("group_size", _i32),
+                ("epsilon", _f32), ("x_row_stride", _i64), ("residual_row_stride", _i64), ("out_row_stride", _i64),
+                ("residual_out_row_stride", _i64), ("x", _vp), ("residual", _vp), ("weight", _vp), ("out", _vp),
+                ("scales", _vp), ("residual_out", _vp)]
+
+
+class RotaryAppendParams(ctypes.Structure):
+    """Mirror of ``B200RotaryAppendParams``."""
+
+    _fields_ = [("num_heads", _i32), ("kv_num_heads", _i32), ("head_size", _i32), ("rotary_dim", _i32),
+                ("rotary_offset", _i32), ("rotary_interleaved", _i32), ("rotary_positions", _i32), ("axes", _i32),
+                ("axis_pairs", _i32 * 4), ("act_dtype", _i32), ("cache_dtype", _i32), ("table_dtype", _i32),
+                ("position_dtype", _i32), ("num_tokens", _i32), ("num_blocks", _i32), ("block_size", _i32),
+                ("query_row_stride", _i64), ("key_row_stride", _i64), ("value_row_stride", _i64),
+                ("output_row_stride", _i64), ("position_axis_stride", _i64), ("position_token_stride", _i64),
+                ("query", _vp), ("key", _vp), ("value", _vp), ("output", _vp), ("key_cache", _vp),
+                ("value_cache", _vp), ("position_ids", _vp), ("cos_cache", _vp), ("sin_cache", _vp),
+                ("slot_mapping", _vp), ("k_scale", _vp), ("v_scale", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t), ("device_status", _vp)]
+
+
+class SharedPrefixParams(ctypes.Structure):
+    """Mirror of ``B200SharedPrefixParams``."""
+
+    _fields_ = [("num_heads", _i32), ("kv_num_heads", _i32), ("head_size", _i32), ("scale", _f32), ("softcap", _f32),
+                ("act_dtype", _i32), ("num_tokens", _i32), ("batch", _i32), ("num_blocks", _i32), ("block_size", _i32),
+                ("max_blocks_per_seq", _i32), ("prefix_length", _i32), ("prefix_blocks", _i32), ("num_sms", _i32),
+                ("query_row_stride", _i64), ("output_row_stride", _i64), ("query", _vp), ("key_cache", _vp),
+                ("value_cache", _vp), ("cumulative_sequence_length", _vp), ("past_seqlens", _vp), ("block_table", _vp),
+                ("prefix_block_table", _vp), ("head_sink", _vp), ("output", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t), ("device_status", _vp)]
+
+
 # Every entry point the headers declare, with its ctypes signature.
 SIGNATURES = {
     "b200_version": (ctypes.c_int, []),
@@ -232,6 +272,14 @@ SIGNATURES = {
     "b200_ipc_get_handle": (ctypes.c_int, [_vp, _vp]),
     "b200_ipc_open_handle": (ctypes.c_int, [_i32, _vp, ctypes.POINTER(_vp)]),
     "b200_ipc_close_handle": (ctypes.c_int, [_i32, _vp]),
+    # include/b200_layer.h (pointers passed as addresses: byref of the params struct)
+    "b200_layer_struct_size": (ctypes.c_size_t, [_i32]),
+    "b200_layer_read_status": (ctypes.c_int, [_vp, _vp]),
+    "b200_skip_rms_norm": (ctypes.c_int, [_vp, _vp]),
+    "b200_rotary_append_workspace_size": (ctypes.c_int, [_vp, _vp]),
+    "b200_rotary_append": (ctypes.c_int, [_vp, _vp]),
+    "b200_shared_prefix_attention_workspace_size": (ctypes.c_int, [_vp, _vp]),
+    "b200_shared_prefix_attention": (ctypes.c_int, [_vp, _vp]),
 }
 
 
@@ -270,6 +318,9 @@ def load() -> ctypes.CDLL:
         raise ImportError("libb200_paged.so: B200ShardGatherParams layout differs from the binding")
     for which, cls in enumerate((EpOptions, KvPoolDesc, KvPoolInfo, PagedTensors)):
         if lib.b200_ep_struct_size(which) != ctypes.sizeof(cls):
+            raise ImportError(f"libb200_paged.so: {cls.__name__} layout differs from the binding")
+    for which, cls in enumerate((SkipRmsNormParams, RotaryAppendParams, SharedPrefixParams)):
+        if lib.b200_layer_struct_size(which) != ctypes.sizeof(cls):
             raise ImportError(f"libb200_paged.so: {cls.__name__} layout differs from the binding")
     return lib
 
