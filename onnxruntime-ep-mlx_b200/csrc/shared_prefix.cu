@@ -1,14 +1,18 @@
 // Causal attention over paged caches for a batch whose sequences share one prefix
-// (b200_shared_prefix_attention).
+// (b200_shared_prefix_attention): the plan and merge kernels of the fast path (shared_prefix.cuh
+// gives its structure), the generic kernel, and the launches.
 //
-// shared_prefix_generic_kernel: a CTA per (token, query head); its warps take every kWarps-th key
+// Softmax over a union of key sets: with M the largest m of a row's triples (m, l, o),
+//   out = sum 2^(m_i - M) o_i / (sum 2^(m_i - M) l_i + 2^(sink log2 e - M))
+//
+// shared_prefix_generic_kernel (any head size up to 256, block size and head ratio): a CTA per (token, query head); its warps take every kWarps-th key
 // of the prefix and of the token's own keys with an fp32 running softmax (m, l, o), and the warps'
-// triples are joined in shared memory.  Any head size up to 256, block size and head ratio.
+// triples are joined in shared memory.
 #include <algorithm>
 #include <cmath>
 
-#include "b200_common.cuh"
-#include "layer_kernels.h"
+#include "b200_kernels.h"
+#include "shared_prefix.cuh"
 
 namespace b200 {
 namespace {
@@ -115,15 +119,314 @@ void launch_generic_t(const B200SharedPrefixParams& p, cudaStream_t stream) {
   else shared_prefix_generic_kernel<T, 8><<<grid, 32 * kGenericWarps, 0, stream>>>(p);
 }
 
+
+// ---------------------------------------------------------------------------------------------
+// Plan: one CTA checks the lengths, routes every sequence and lays out both work lists.
+// ---------------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+
+// Inclusive sums of (x, y) over the block, totals in `total`.
+__device__ __forceinline__ int2 block_inclusive_sum(int2 v, int2* warp_sums, int2& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, v.x, o), y = __shfl_up_sync(0xffffffffu, v.y, o);
+    if (lane >= o) {
+      v.x += x;
+      v.y += y;
+    }
+  }
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    int2 s = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, s.x, o), y = __shfl_up_sync(0xffffffffu, s.y, o);
+      if (lane >= o) {
+        s.x += x;
+        s.y += y;
+      }
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  if (warp > 0) {
+    v.x += warp_sums[warp - 1].x;
+    v.y += warp_sums[warp - 1].y;
+  }
+  total = warp_sums[31];
+  __syncthreads();
+  return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const SharedPrefixArgs a) {
+  __shared__ int2 warp_sums[32];
+  const B200SharedPrefixParams& p = a.p;
+  release_dependents();
+  const int tid = threadIdx.x, lane = tid & 31;
+  for (int t = tid; t < p.num_tokens; t += kPlanThreads) a.token_seq[t] = -1;
+  if (tid == 0) *a.next_item = 0;
+  __syncthreads();
+  int2 carry = make_int2(0, 0);
+  for (int base = 0; base < p.batch; base += kPlanThreads) {
+    const int b = base + tid;
+    int2 work = make_int2(0, 0);  // 16-key tiles of the own kernel, query-tile pairs of the tensor-core kernel
+    int c0 = 0, nq = 0;
+    if (b < p.batch) {
+      c0 = p.cumulative_sequence_length[b];
+      const int c1 = p.cumulative_sequence_length[b + 1], past = p.past_seqlens[b];
+      const int64_t total = (int64_t)past + c1 - c0;
+      int bits = 0;
+      if (c0 < 0 || c0 > c1 || c1 > p.num_tokens || (b == 0 && c0 != 0) || (b == p.batch - 1 && c1 != p.num_tokens))
+        bits |= kStatusBadCumulative;
+      if (past < 0) bits |= kStatusBadPast;
+      if (total > (int64_t)p.max_blocks_per_seq * p.block_size) bits |= kStatusBadCapacity;
+      if (bits) set_status(p.device_status, bits);
+      if (c0 >= 0 && c0 <= c1 && c1 <= p.num_tokens && past >= 0 && !(bits & kStatusBadCapacity)) nq = c1 - c0;
+      if ((int64_t)nq * a.group <= a.own_rows) work.x = nq ? (int)((total + kOwnTile - 1) / kOwnTile) : 0;
+      else work.y = (nq + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
+    }
+    if (nq <= 32)
+      for (int i = 0; i < nq; ++i) a.token_seq[c0 + i] = b;
+    for (unsigned left = __ballot_sync(0xffffffffu, nq > 32); left; left &= left - 1) {  // long ones: the whole warp
+      const int src = __ffs(left) - 1;
+      const int first = __shfl_sync(0xffffffffu, c0, src), n = __shfl_sync(0xffffffffu, nq, src);
+      const int seq = __shfl_sync(0xffffffffu, b, src);
+      for (int i = lane; i < n; i += 32) a.token_seq[first + i] = seq;
+    }
+    int2 total;
+    const int2 incl = block_inclusive_sum(work, warp_sums, total);
+    if (b < p.batch) {
+      a.seq_tiles[b] = carry.x + incl.x - work.x;
+      a.seq_pairs[b] = carry.y + incl.y - work.y;
+    }
+    carry.x += total.x;
+    carry.y += total.y;
+  }
+  if (tid == 0) {
+    a.seq_tiles[p.batch] = carry.x;
+    a.seq_pairs[p.batch] = carry.y;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Merge: one warp per (token, head) row joins the row's triples.
+// ---------------------------------------------------------------------------------------------
+constexpr int kMergeWarps = 8;
+constexpr float kLog2eMerge = 1.4426950408889634f;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kMergeWarps) shared_prefix_merge_kernel(const SharedPrefixArgs a, int vector_rows) {
+  constexpr int C = D / 32;  // channels per lane
+  const B200SharedPrefixParams& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  wait_previous();
+  if (row >= a.rows) return;
+  const int64_t t = row / p.num_heads;
+  const int h = (int)(row % p.num_heads), kh = h / a.group;
+  // own part: the slab, or `pieces` warps' rows
+  const int b = a.token_seq[t];
+  int own = 0;  // triples of the own keys
+  bool cut = false;
+  int64_t w_first = 0, first_row = 0, next_row = 0;
+  if (b >= 0) {
+    own = 1;
+    const int c0 = p.cumulative_sequence_length[b], nq = p.cumulative_sequence_length[b + 1] - c0;
+    if ((int64_t)nq * a.group <= a.own_rows) {
+      const int KV = p.kv_num_heads;
+      const int64_t first = a.seq_tiles[b], tiles = a.seq_tiles[b + 1] - first;
+      const int64_t T_all = (int64_t)a.seq_tiles[p.batch] * KV, W = own_active_warps(T_all, a.own_warps);
+      const int64_t start = first * KV + kh * tiles;
+      w_first = own_warp_of(start, T_all, W);
+      own = (int)(own_warp_of(start + tiles - 1, T_all, W) - w_first + 1);
+      cut = own > 1;
+      // a warp's row block 0 holds the piece its range starts with, block 1 its last one
+      const int64_t r = (t - c0) * a.group + h % a.group;
+      first_row = (w_first * 2 + (start > own_range_start(w_first, T_all, W) ? 1 : 0)) * a.own_rows + r;
+      next_row = (w_first + 1) * 2 * a.own_rows + r;
+    }
+  }
+  const int parts = a.splits + own;
+  auto locate = [&](int i) -> int64_t {  // row of triple i in its array; cut pieces are i >= splits
+    if (!cut || i < a.splits) return (int64_t)i * a.rows + row;
+    const int piece = i - a.splits;
+    return piece == 0 ? first_row : next_row + (int64_t)(piece - 1) * 2 * a.own_rows;
+  };
+  auto triple = [&](int i) -> float2 {
+    return __ldcg((cut && i >= a.splits ? a.warp_ml : a.slab_ml) + locate(i));
+  };
+  const float sink = p.head_sink ? act<T>::to_f(static_cast<const T*>(p.head_sink)[h]) * kLog2eMerge : -INFINITY;
+  float top = sink;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, triple(i).x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (top == -INFINITY) top = 0.f;
+  float sum = 0.f, acc[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) acc[c] = 0.f;
+  for (int base = 0; base < parts; base += 32) {
+    float weight = 0.f;
+    if (base + lane < parts) {
+      const float2 ml = triple(base + lane);
+      weight = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+      sum += ml.y * weight;
+    }
+    const int n = min(32, parts - base);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float f = __shfl_sync(0xffffffffu, weight, j);
+      const int i = base + j;
+      const float* src = (cut && i >= a.splits ? a.warp_o : a.slab_o) + locate(i) * D + lane * C;
+      if constexpr (C == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+        if (f != 0.f) {
+          acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
+        }
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+        if (f != 0.f) {
+          acc[0] += f * v.x; acc[1] += f * v.y;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (p.head_sink) sum += exp2f(sink - top);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* out = static_cast<T*>(p.output) + t * p.output_row_stride + (int64_t)h * D + lane * C;
+  if (vector_rows) {
+    uint32_t w[C / 2];
+#pragma unroll
+    for (int c = 0; c < C / 2; ++c) w[c] = mma_op<T>::pack(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+    if constexpr (C == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(out) = w[0];
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) out[c] = act<T>::from_f(acc[c] * inv);
+  }
+}
+
+template <typename T>
+cudaError_t launch_merge_t(const SharedPrefixArgs& a, cudaStream_t stream) {
+  const bool vec = (reinterpret_cast<uintptr_t>(a.p.output) | (uintptr_t)(a.p.output_row_stride * 2)) % 8 == 0;
+  const dim3 grid((unsigned)((a.rows + kMergeWarps - 1) / kMergeWarps)), block(32 * kMergeWarps);
+  return a.p.head_size == 64 ? launch_dependent(shared_prefix_merge_kernel<T, 64>, grid, block, 0, stream, a, (int)vec)
+                             : launch_dependent(shared_prefix_merge_kernel<T, 128>, grid, block, 0, stream, a, (int)vec);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side of the fast path
+// ---------------------------------------------------------------------------------------------
+// The shapes the fast path covers; the call also needs 16-byte rows (fast_rows).
+bool fast_shape(const B200SharedPrefixParams& p) {
+  return (p.head_size == 64 || p.head_size == 128) && p.block_size % kOwnTile == 0 &&
+         p.num_heads / p.kv_num_heads <= 128;
+}
+
+bool fast_rows(const B200SharedPrefixParams& p) {
+  return ((reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.key_cache) |
+           reinterpret_cast<uintptr_t>(p.value_cache) | (uintptr_t)(p.query_row_stride * 2)) & 15) == 0;
+}
+
+// Key ranges of the prefix: the fewest "tile times" over waves of the SMs, where an item costs its
+// tiles plus about 2 for its start and end, and a further range costs its rows' triples to write and
+// read (about 12 TB/s of traffic against 2.5 us a tile).
+void split_prefix(SharedPrefixArgs* a, int num_sms) {
+  const B200SharedPrefixParams& p = a->p;
+  const int64_t tiles = ((int64_t)p.prefix_length + kPrefixKeys - 1) / kPrefixKeys;
+  const int64_t items = (int64_t)p.kv_num_heads * a->query_pairs;
+  a->splits = 0;
+  a->split_tiles = 1;
+  if (tiles == 0 || items == 0) return;
+  const double per_range = (double)a->rows * p.head_size * 8 / 12e12 / 2.5e-6;
+  double best = 0;
+  for (int64_t s = 1; s <= 64 && s <= tiles; ++s) {
+    const int64_t per = (tiles + s - 1) / s, n = (tiles + per - 1) / per;
+    const double cost = (double)((items * n + num_sms - 1) / num_sms) * (per + 2) + per_range * n;
+    if (a->splits == 0 || cost < best) {
+      best = cost;
+      a->splits = (int)n;
+      a->split_tiles = (int)per;
+    }
+  }
+}
+
+// Fills `a` and returns the workspace bytes (0: generic kernel).
+size_t layout(const B200SharedPrefixParams& p, int num_sms, SharedPrefixArgs* a) {
+  if (!fast_shape(p) || p.num_tokens == 0) return 0;
+  a->p = p;
+  a->group = p.num_heads / p.kv_num_heads;
+  a->tile_tokens = 128 / a->group;
+  a->query_pairs = (p.num_tokens + 2 * a->tile_tokens - 1) / (2 * a->tile_tokens);
+  // one 8-row MMA tile when a kv head's rows of one token fit and sequences have about one token
+  a->own_rows = a->group <= 8 && p.num_tokens <= p.batch ? 8 : 16;
+  a->own_warps = num_sms * kOwnCtasPerSm * kOwnWarps;
+  a->rows = (int64_t)p.num_tokens * p.num_heads;
+  split_prefix(a, num_sms);
+  char* base = static_cast<char*>(p.workspace);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* at = base + off;
+    off = (off + bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t d = p.head_size, slabs = (size_t)a->splits + 1, wrows = (size_t)a->own_warps * 2 * a->own_rows;
+  a->next_item = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long)));
+  a->seq_tiles = reinterpret_cast<int*>(take(sizeof(int) * ((size_t)p.batch + 1)));
+  a->seq_pairs = reinterpret_cast<int*>(take(sizeof(int) * ((size_t)p.batch + 1)));
+  a->token_seq = reinterpret_cast<int*>(take(sizeof(int) * (size_t)p.num_tokens));
+  a->slab_ml = reinterpret_cast<float2*>(take(sizeof(float2) * slabs * a->rows));
+  a->warp_ml = reinterpret_cast<float2*>(take(sizeof(float2) * wrows));
+  a->slab_o = reinterpret_cast<float*>(take(sizeof(float) * slabs * a->rows * d));
+  a->warp_o = reinterpret_cast<float*>(take(sizeof(float) * wrows * d));
+  return off;
+}
+
+cudaError_t encode_maps(const SharedPrefixArgs& a, SharedPrefixMaps* maps) {
+  const B200SharedPrefixParams& p = a.p;
+  const bool bf = p.act_dtype == B200_DTYPE_BFLOAT16;
+  const uint64_t d = p.head_size, kv = p.kv_num_heads;
+  const uint64_t dims[3] = {d, kv, (uint64_t)p.num_blocks * p.block_size}, strides[2] = {d * 2, kv * d * 2};
+  const uint32_t box[3] = {64, 1, kOwnTile};
+  const uint64_t q_dims[3] = {d, (uint64_t)p.num_heads, (uint64_t)p.num_tokens};
+  const uint64_t q_strides[2] = {d * 2, (uint64_t)p.query_row_stride * 2};
+  const uint32_t q_box[3] = {64, (uint32_t)a.group, (uint32_t)a.tile_tokens};
+  if (encode_tensor_map(&maps->k_map, bf, 3, p.key_cache, dims, strides, box) ||
+      encode_tensor_map(&maps->v_map, bf, 3, p.value_cache, dims, strides, box) ||
+      encode_tensor_map(&maps->q_map, bf, 3, p.query, q_dims, q_strides, q_box))
+    return cudaErrorInvalidValue;
+  return cudaSuccess;
+}
+
 }  // namespace
 
-size_t shared_prefix_workspace(const B200SharedPrefixParams&, int) { return 0; }
+size_t shared_prefix_workspace(const B200SharedPrefixParams& p, int num_sms) {
+  SharedPrefixArgs a{};
+  return layout(p, num_sms, &a);
+}
 
-cudaError_t launch_shared_prefix(const B200SharedPrefixParams& p, int, cudaStream_t stream) {
-  if (p.act_dtype == B200_DTYPE_BFLOAT16) launch_generic_t<__nv_bfloat16>(p, stream);
-  else launch_generic_t<__half>(p, stream);
-  add_launches(1);
-  return cudaGetLastError();
+cudaError_t launch_shared_prefix(const B200SharedPrefixParams& p, int num_sms, cudaStream_t stream) {
+  SharedPrefixArgs a{};
+  if (layout(p, num_sms, &a) == 0 || !fast_rows(p)) {
+    if (p.act_dtype == B200_DTYPE_BFLOAT16) launch_generic_t<__nv_bfloat16>(p, stream);
+    else launch_generic_t<__half>(p, stream);
+    add_launches(1);
+    return cudaGetLastError();
+  }
+  SharedPrefixMaps maps;
+  cudaError_t e = encode_maps(a, &maps);
+  if (e != cudaSuccess) return e;
+  shared_prefix_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+  e = cudaGetLastError();
+  if (e == cudaSuccess) e = launch_shared_prefix_tc(a, maps, num_sms, stream);
+  if (e == cudaSuccess) e = launch_shared_prefix_own(a, maps, stream);
+  if (e == cudaSuccess)
+    e = p.act_dtype == B200_DTYPE_BFLOAT16 ? launch_merge_t<__nv_bfloat16>(a, stream) : launch_merge_t<__half>(a, stream);
+  if (e == cudaSuccess) add_launches(4);
+  return e;
 }
 
 }  // namespace b200

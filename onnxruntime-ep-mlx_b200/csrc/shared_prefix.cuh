@@ -1,0 +1,88 @@
+// Shared pieces of the fast path of b200_shared_prefix_attention: its plan in the workspace, the
+// argument block and programmatic dependent launch.
+//
+// One call is four launches:
+//   shared_prefix_plan_kernel   lengths -> work lists (1 CTA)
+//   shared_prefix_tc_kernel     tensor-core pass (tcgen05): every token against a range of the
+//                               prefix's keys, and long chunks against their own keys
+//   shared_prefix_own_kernel    single tokens and short chunks against their own keys (memory bound)
+//   shared_prefix_merge_kernel  joins the softmax triples (m, l, o) of each (token, head) row
+// The passes leave unnormalised fp32 o with m (log2 domain) and l: prefix range s of the S ranges in
+// slab s, own keys in slab S, each slab [num_tokens * num_heads][head_size]; own keys that stream-K
+// cut between warps stay in the warps' own rows until the merge.
+#pragma once
+
+#include <utility>
+
+#include "b200_common.cuh"
+#include "layer_kernels.h"
+
+namespace b200 {
+
+struct SharedPrefixArgs {
+  B200SharedPrefixParams p;
+  int group;         // query heads per kv head
+  int tile_tokens;   // tokens of one 128-row query tile: 128 / group
+  int splits;        // S: key ranges of the prefix
+  int split_tiles;   // 128-key tiles per range
+  int query_pairs;   // pairs of query tiles over all tokens
+  int own_rows;      // sequences of at most this many (token, head-in-group) rows: own kernel
+  int own_warps;     // warps of the own kernel's grid
+  int64_t rows;      // num_tokens * num_heads
+  // plan
+  int* seq_tiles;    // [batch + 1] exclusive prefix of 16-key tiles (per kv head), own kernel
+  int* seq_pairs;    // [batch + 1] exclusive prefix of query-tile pairs, tensor-core kernel
+  int* token_seq;    // [num_tokens] sequence of a token, -1 without a valid one
+  unsigned long long* next_item;  // tensor-core work list position
+  // partials
+  float* slab_o;     // [splits + 1][rows][head_size]
+  float2* slab_ml;   // [splits + 1][rows]
+  float* warp_o;     // [own_warps * 2][own_rows][head_size]
+  float2* warp_ml;   // [own_warps * 2][own_rows]
+};
+
+struct SharedPrefixMaps {
+  CUtensorMap k_map, v_map;  // [num_blocks * block_size, kv heads, d]: box {64, 1, 16}
+  CUtensorMap q_map;         // [tokens, heads, d]: box {64, group, tile_tokens}
+};
+
+constexpr int kOwnTile = 16;  // keys per tile of the own kernel
+constexpr int kOwnWarps = 4;  // warps per CTA
+constexpr int kOwnCtasPerSm = 2;  // its shared memory, 97 KB per CTA, leaves room for two
+constexpr int kPrefixKeys = 128;  // keys per tile of the tensor-core kernel
+
+cudaError_t launch_shared_prefix_tc(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms,
+                                    cudaStream_t stream);
+cudaError_t launch_shared_prefix_own(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, cudaStream_t stream);
+
+// Stream-K ranges of the own kernel: warp w of W owns tiles [start(w), start(w + 1)) of T.
+__host__ __device__ __forceinline__ int64_t own_range_start(int64_t w, int64_t T, int64_t W) { return w * T / W; }
+__device__ __forceinline__ int64_t own_warp_of(int64_t x, int64_t T, int64_t W) { return ((x + 1) * W + T - 1) / T - 1; }
+// Warps that share T tiles: all of them, but at least 4 tiles each.
+__device__ __forceinline__ int64_t own_active_warps(int64_t T, int64_t grid_warps) {
+  const int64_t most = (T + 3) / 4;
+  return most < 1 ? 1 : (most < grid_warps ? most : grid_warps);
+}
+
+// Programmatic dependent launch: a kernel launched with the attribute may start once every CTA of
+// the previous one has called release_dependents() (or exited); wait_previous() returns when the
+// previous kernel has completed and its writes are visible.
+__device__ __forceinline__ void release_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+
+}  // namespace b200

@@ -1,0 +1,374 @@
+// shared_prefix_own_kernel: single new tokens and short chunks (at most own_rows = 8 NT rows of a kv
+// head) against their sequence's own keys.
+//
+// Bound by HBM: every own key is read once per call and serves the few rows of its kv head (2 g
+// flops per byte).  All own keys of these sequences form one stream of 16-key tiles (sequence, kv
+// head, tile); each warp of the persistent grid owns an equal contiguous range of it, so ragged
+// lengths balance exactly.  A warp streams its tiles through a private ring of shared-memory stages
+// filled by TMA (128-byte swizzle), the lookahead running across sequence boundaries.  Per tile:
+//   S^T[16 keys x 8 NT rows] = K . Q^T       mma.m16n8k16, K by ldmatrix, Q in registers
+//   softmax with a running maximum           fp32, exp2 domain
+//   O^T[d x 8 NT rows] += V^T . P^T          ldmatrix.trans; P as a hi + lo pair of 16-bit values
+// (a 128-row tcgen05 tile would be empty but for these rows and the tensor pipe is not the bound).
+// A (sequence, kv head) segment inside one warp's range goes to the own slab; a cut one leaves a
+// triple per warp, at most two per warp, for the merge kernel.
+#include <atomic>
+
+#include "shared_prefix.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct OwnLayout {
+  static constexpr int kBoxes = D / 64;
+  static constexpr int kBoxBytes = kOwnTile * 128;
+  static constexpr int kTileBytes = kBoxes * kBoxBytes;
+  static constexpr int kStageBytes = 2 * kTileBytes;  // K and V
+  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kSmem = kOwnWarps * kStages * kStageBytes + 1024;
+};
+
+// 16-byte piece `chunk` of tile row `row` in the 128B-swizzled boxes.
+__device__ __forceinline__ uint32_t own_swizzle(int row, int chunk) {
+  return (uint32_t)((chunk >> 3) * (kOwnTile * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// A part of one (sequence, kv head) segment of the tile stream.
+struct Piece {
+  int valid, b, kh, t0, t1, tiles, c0, nq, past, total;
+  int64_t seg_start;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const __grid_constant__ SharedPrefixArgs a,
+                                                                            const __grid_constant__ SharedPrefixMaps maps) {
+  using L = OwnLayout<D>;
+  using MMA = mma_op<T>;
+  constexpr int KSTEPS = D / 16, STAGES = L::kStages, RING = STAGES + 1, ROWS = 8 * NT;
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ __align__(8) uint64_t bars[kOwnWarps][STAGES];
+  __shared__ Piece ring[kOwnWarps][RING];
+
+  release_dependents();
+  const B200SharedPrefixParams& p = a.p;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* wbase = smem + warp * STAGES * L::kStageBytes;
+  const uint32_t wbase_u32 = smem_u32(wbase);
+  Piece* myring = ring[warp];
+
+  const int KV = p.kv_num_heads, g = a.group, H = p.num_heads;
+  // The plan is complete: this grid starts after every CTA of the tensor-core kernel has waited for it.
+  const int64_t total_tiles = (int64_t)__ldcg(a.seq_tiles + p.batch) * KV;
+  const int64_t W = own_active_warps(total_tiles, a.own_warps);
+  const int64_t gw = (int64_t)blockIdx.x * kOwnWarps + warp;
+  const int64_t r0 = gw < W ? own_range_start(gw, total_tiles, W) : 0;
+  const int64_t r1 = gw < W ? own_range_start(gw + 1, total_tiles, W) : 0;
+  if (r0 >= r1) {
+    wait_previous();  // this grid's completion stands for the tensor-core kernel's, too
+    return;
+  }
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(&bars[warp][s], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  const float qk_scale = p.softcap > 0.f ? p.scale : p.scale * kLog2e;
+
+  // The piece at stream position x (< r1) into ring slot `slot`.
+  auto locate = [&](int slot, int64_t x) {
+    Piece u{};
+    if (x < r1) {
+      int lo = 0, hi = p.batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((int64_t)__ldcg(a.seq_tiles + mid) * KV <= x) lo = mid; else hi = mid - 1;
+      }
+      const int first = __ldcg(a.seq_tiles + lo), tiles = __ldcg(a.seq_tiles + lo + 1) - first;
+      if (tiles > 0) {
+        const int64_t rel = x - (int64_t)first * KV;
+        u.valid = 1;
+        u.b = lo;
+        u.kh = (int)(rel / tiles);
+        u.tiles = tiles;
+        u.t0 = (int)(rel % tiles);
+        u.t1 = (int)min((int64_t)tiles, u.t0 + (r1 - x));
+        u.seg_start = (int64_t)first * KV + (int64_t)u.kh * tiles;
+        u.c0 = p.cumulative_sequence_length[lo];
+        u.nq = p.cumulative_sequence_length[lo + 1] - u.c0;
+        u.past = p.past_seqlens[lo];
+        u.total = u.past + u.nq;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) myring[slot] = u;
+    __syncwarp();
+  };
+
+  auto issue = [&](int s, int slot, int t) {  // lane 0: the TMA loads of tile t into stage s
+    if (lane != 0) return;
+    const Piece& u = myring[slot];
+    uint64_t* bar = &bars[warp][s];
+    const int pos = t * kOwnTile;
+    const int32_t blk = p.block_table[(int64_t)u.b * p.max_blocks_per_seq + pos / p.block_size];
+    if (blk < 0 || blk >= p.num_blocks) {
+      set_status(p.device_status, kStatusBadBlock);
+      mbar_arrive(bar);
+      return;
+    }
+    const int z = blk * p.block_size + pos % p.block_size;
+    uint8_t* kdst = wbase + s * L::kStageBytes;
+    mbar_arrive_expect_tx(bar, L::kStageBytes);
+#pragma unroll
+    for (int h = 0; h < L::kBoxes; ++h) {
+      tma_load_3d(kdst + h * L::kBoxBytes, &maps.k_map, bar, h * 64, u.kh, z);
+      tma_load_3d(kdst + L::kTileBytes + h * L::kBoxBytes, &maps.v_map, bar, h * 64, u.kh, z);
+    }
+  };
+
+  int ps = 0, pt = 0;
+  locate(0, r0);
+  bool producing = myring[0].valid != 0;
+  if (producing) pt = myring[0].t0;
+  uint32_t phase = 0, pending = 0;
+  int issued = 0, consumed = 0;
+  bool failed = false;
+  auto produce = [&]() {
+    while (producing && pt >= myring[ps].t1) {
+      const int64_t next = myring[ps].seg_start + myring[ps].t1;
+      ps = (ps + 1) % RING;
+      locate(ps, next);
+      producing = myring[ps].valid != 0;
+      if (producing) pt = myring[ps].t0;
+    }
+    if (!producing) return;
+    const int s = issued % STAGES;
+    issue(s, ps, pt);
+    pending |= 1u << s;
+    ++pt;
+    ++issued;
+  };
+  for (int i = 0; i < STAGES; ++i) produce();
+  __syncwarp();
+
+  int cs = 0, ct = myring[0].t0;
+  const int col0 = (lane & 3) * 2;  // rows held by this lane: 8 n + col0, + 1
+
+  while (consumed < issued && !failed) {
+    const Piece u = myring[cs];
+    const int rows = u.nq * g;
+
+    // Q^T fragments: column lane / 4 of n-tile n is row 8 n + lane / 4 = (token, head in group)
+    uint32_t qf[NT][KSTEPS][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = 8 * n + (lane >> 2), kq = (lane & 3) * 2;
+      const bool in = r < rows;
+      const T* qrow = static_cast<const T*>(p.query) + (int64_t)(u.c0 + (in ? r / g : 0)) * p.query_row_stride +
+                      (int64_t)(u.kh * g + (in ? r % g : 0)) * D;
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        qf[n][kk][0] = in ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16 + kq) : 0u;
+        qf[n][kk][1] = in ? *reinterpret_cast<const uint32_t*>(qrow + kk * 16 + 8 + kq) : 0u;
+      }
+    }
+    float m[NT][2], l[NT][2], o[NT][KSTEPS][4];
+    int limit[NT][2];  // last own key the row sees; -1: no such row
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * n + col0 + e;
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+        limit[n][e] = r < rows ? u.past + r / g : -1;
+      }
+#pragma unroll
+      for (int mt = 0; mt < KSTEPS; ++mt) o[n][mt][0] = o[n][mt][1] = o[n][mt][2] = o[n][mt][3] = 0.f;
+    }
+    // block ids of 32 tiles at a time: lane i holds tile wb + i's, the next window loaded ahead
+    auto tile_block = [&](int t) -> int32_t {
+      return t < u.t1 ? __ldg(p.block_table + (int64_t)u.b * p.max_blocks_per_seq + t * kOwnTile / p.block_size) : -1;
+    };
+    int wb = ct;
+    int32_t w_blk = tile_block(wb + lane), n_blk = -1;
+
+    for (; ct < u.t1; ++ct) {
+      const int s = consumed % STAGES;
+      const int pos0 = ct * kOwnTile;
+      int wi = ct - wb;
+      if (wi == 32) {
+        wb = ct;
+        wi = 0;
+        w_blk = n_blk;
+      }
+      if (wi == 0) n_blk = tile_block(wb + 32 + lane);
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars[warp][s], (phase >> s) & 1u))) {
+        if (lane == 0) set_status(p.device_status, kStatusTimeout);
+        failed = true;
+        for (int s2 = 0; s2 < STAGES; ++s2)  // one more bounded wait for the loads in flight
+          if ((pending >> s2) & 1u) mbar_wait(&bars[warp][s2], (phase >> s2) & 1u);
+        break;
+      }
+      phase ^= 1u << s;
+      pending &= ~(1u << s);
+      const int32_t blk = __shfl_sync(0xffffffffu, w_blk, wi);
+      const bool blk_ok = blk >= 0 && blk < p.num_blocks;
+      const bool full = blk_ok && pos0 + kOwnTile <= u.past + 1;  // every row sees every key
+      const uint32_t kbase = wbase_u32 + s * L::kStageBytes, vbase = kbase + L::kTileBytes;
+      const bool tail = pos0 + kOwnTile > u.total;
+      if (tail || !blk_ok) {
+        // V rows of unused slots become zeros: 0 x NaN from whatever they hold would poison o
+        const int first = blk_ok ? u.total - pos0 : 0;
+        for (int i = lane; i < (kOwnTile - first) * (D / 8); i += 32)
+          *reinterpret_cast<uint4*>(wbase + (vbase - wbase_u32) + own_swizzle(first + i / (D / 8), i % (D / 8))) =
+              make_uint4(0u, 0u, 0u, 0u);
+        __syncwarp();
+      }
+
+      float c[NT][2][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) c[n][j][0] = c[n][j][1] = c[n][j][2] = c[n][j][3] = 0.f;
+      {
+        const int row = (lane & 7) + ((lane >> 3) & 1) * 8, half = lane >> 4;
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; kk += 2) {
+          uint32_t af[4], bf[4];
+          ldsm_x4(kbase + own_swizzle(row, kk * 2 + half), af[0], af[1], af[2], af[3]);
+          ldsm_x4(kbase + own_swizzle(row, kk * 2 + 2 + half), bf[0], bf[1], bf[2], bf[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            MMA::run(c[n][0], af, qf[n][kk][0], qf[n][kk][1]);
+            MMA::run(c[n][1], bf, qf[n][kk + 1][0], qf[n][kk + 1][1]);
+          }
+        }
+      }
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float sc[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int pos = pos0 + (lane >> 2) + ((e >> 1) << 3);
+          float x = (c[n][0][e] + c[n][1][e]) * qk_scale;
+          if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap) * kLog2e;
+          const bool seen = full ? limit[n][e & 1] >= 0 : blk_ok && pos <= limit[n][e & 1];
+          sc[e] = seen ? x : -INFINITY;
+        }
+        float mx0 = fmaxf(sc[0], sc[2]), mx1 = fmaxf(sc[1], sc[3]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+        }
+        const float mn0 = fmaxf(m[n][0], mx0), mn1 = fmaxf(m[n][1], mx1);
+        const float mu0 = mn0 == -INFINITY ? 0.f : mn0, mu1 = mn1 == -INFINITY ? 0.f : mn1;
+        const float al0 = exp2f(m[n][0] - mu0), al1 = exp2f(m[n][1] - mu1);
+        const float p0 = exp2f(sc[0] - mu0), p1 = exp2f(sc[1] - mu1);
+        const float p2 = exp2f(sc[2] - mu0), p3 = exp2f(sc[3] - mu1);
+        l[n][0] = l[n][0] * al0 + p0 + p2;
+        l[n][1] = l[n][1] * al1 + p1 + p3;
+        m[n][0] = mn0;
+        m[n][1] = mn1;
+#pragma unroll
+        for (int mt = 0; mt < KSTEPS; ++mt) {
+          o[n][mt][0] *= al0; o[n][mt][2] *= al0;
+          o[n][mt][1] *= al1; o[n][mt][3] *= al1;
+        }
+        // P to 16 bits twice: the rounded value and what the rounding left (about 16 bits in all)
+        const uint32_t x0 = MMA::pack(p0, p1), x1 = MMA::pack(p2, p3);
+        const float2 h0 = MMA::unpack(x0), h1 = MMA::unpack(x1);
+        ph[n][0] = movm_t(x0);
+        ph[n][1] = movm_t(x1);
+        pl[n][0] = movm_t(MMA::pack(p0 - h0.x, p1 - h0.y));
+        pl[n][1] = movm_t(MMA::pack(p2 - h1.x, p3 - h1.y));
+      }
+      {
+        const int jm = lane >> 3;
+        const int row = (lane & 7) + (jm >> 1) * 8, sub = jm & 1;
+#pragma unroll
+        for (int mt = 0; mt < KSTEPS; ++mt) {
+          uint32_t af[4];
+          ldsm_x4_t(vbase + own_swizzle(row, mt * 2 + sub), af[0], af[1], af[2], af[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            MMA::run(o[n][mt], af, ph[n][0], ph[n][1]);
+            MMA::run(o[n][mt], af, pl[n][0], pl[n][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (tail || !blk_ok) fence_proxy_async_smem();  // the zeros before the next TMA write
+      __syncwarp();
+      ++consumed;
+      produce();
+      __syncwarp();
+    }
+    if (failed) break;
+
+    // the piece's triples: column sums of l, then the own slab or this warp's rows
+    const int dr = lane >> 2;
+    const bool whole = u.t0 == 0 && u.t1 == u.tiles;
+    // slot 0: the warp's first piece, slot 1: its last one
+    const int64_t wrow = (gw * 2 + (u.seg_start + u.t0 == r0 ? 0 : 1)) * ROWS;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], off);
+        l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], off);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * n + col0 + e;
+        if (r >= rows) continue;
+        const int64_t row = whole ? (int64_t)a.splits * a.rows + (int64_t)(u.c0 + r / g) * H + u.kh * g + r % g : wrow + r;
+        float* po = (whole ? a.slab_o : a.warp_o) + row * D;
+        if (dr == 0) (whole ? a.slab_ml : a.warp_ml)[row] = make_float2(m[n][e], l[n][e]);
+#pragma unroll
+        for (int mt = 0; mt < KSTEPS; ++mt) {
+          po[mt * 16 + dr] = o[n][mt][e];
+          po[mt * 16 + dr + 8] = o[n][mt][e + 2];
+        }
+      }
+    }
+    cs = (cs + 1) % RING;
+    ct = myring[cs].t0;
+  }
+  wait_previous();  // this grid's completion stands for the tensor-core kernel's, too
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch_own_t(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, cudaStream_t stream) {
+  auto kernel = shared_prefix_own_kernel<T, D, NT>;
+  static std::atomic<uint32_t> ready[64];  // per device: attribute set
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!ready[dev & 63].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnLayout<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    ready[dev & 63].store(1, std::memory_order_release);
+  }
+  return launch_dependent(kernel, dim3(a.own_warps / kOwnWarps), dim3(32 * kOwnWarps),
+                          OwnLayout<D>::kSmem, stream, a, maps);
+}
+
+}  // namespace
+
+cudaError_t launch_shared_prefix_own(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, cudaStream_t stream) {
+  const bool bf = a.p.act_dtype == B200_DTYPE_BFLOAT16, wide = a.own_rows > 8;
+  if (a.p.head_size == 64) {
+    if (bf) return wide ? launch_own_t<__nv_bfloat16, 64, 2>(a, maps, stream) : launch_own_t<__nv_bfloat16, 64, 1>(a, maps, stream);
+    return wide ? launch_own_t<__half, 64, 2>(a, maps, stream) : launch_own_t<__half, 64, 1>(a, maps, stream);
+  }
+  if (bf) return wide ? launch_own_t<__nv_bfloat16, 128, 2>(a, maps, stream) : launch_own_t<__nv_bfloat16, 128, 1>(a, maps, stream);
+  return wide ? launch_own_t<__half, 128, 2>(a, maps, stream) : launch_own_t<__half, 128, 1>(a, maps, stream);
+}
+
+}  // namespace b200

@@ -1,0 +1,557 @@
+// shared_prefix_tc_kernel: the tensor-core (tcgen05) pass of b200_shared_prefix_attention.
+//
+// Work items:
+//   * prefix: (key range, kv head, pair of query tiles): every packed token of the batch against one
+//     range of the shared prefix, without masks.  All tokens and the g query heads of a kv head are
+//     rows of one matrix, so a K/V tile loaded once serves 2 x 128 rows whatever sequences they
+//     belong to;
+//   * chunk: (sequence, kv head, pair of query tiles) of a long chunk against its own keys, causal.
+// Bound by the tensor pipe and the exponentials (4 d flops per row and key); K/V tiles come from L2
+// when more than one pair of query tiles reads a range.
+//
+// A query tile is 128 rows = tile_tokens tokens x g heads.  Roles, joined by mbarriers only:
+//   warps 0-3 / 4-7  softmax and epilogue of query tile 0 / 1, one row per thread = tensor-memory lane
+//   warp 8           takes items, loads Q and K tiles by TMA (8 pages of 16 slots per 128-key tile)
+//   warp 9           issues the MMAs: per K/V tile j PV0(j-1), S0(j), PV1(j-1), S1(j), so the tensor
+//                    pipe works on one query tile while the other one's softmax runs
+//   warp 10          loads V tiles
+// S = Q K^T (both operands in shared memory), O += P V with P in tensor memory over S's columns (fp16:
+// one value per key; bf16: a hi + lo pair, since one bf16 P costs up to 3e-3 on unit-scale values)
+// and V as the MN-major operand in the cache's [key][channel] order.  The running maximum moves, and
+// O is rescaled, only when it grows by more than 2^8.  Tensor memory: S/P 0 and 1 at columns 0 and
+// 128, O 0 and 1 at 256 and 384.  Each item leaves its rows' (m, l, o) in a slab.
+// Every wait is bounded; one that runs out sets the status word, the roles drain what they issued,
+// tensor memory is freed and the kernel returns.
+#include <atomic>
+#include <type_traits>
+
+#include "b200_kernels.h"
+#include "b200_tcgen05.cuh"
+#include "shared_prefix.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kBM = 128;            // query rows per tile
+constexpr int kBN = kPrefixKeys;    // keys per tile
+constexpr int kPage = 16;           // slots per TMA box
+constexpr int kBoxBytes = 128 * 128;  // [128 rows][64 channels]
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kPolyEvery = 4;       // every 4th exponential pair on the FMA pipe
+
+template <int D>
+struct TcLayout {
+  static constexpr int kBoxes = D / 64;
+  static constexpr int kTile = kBoxes * kBoxBytes;
+  static constexpr int kKStages = D == 64 ? 4 : 2;
+  static constexpr int kVStages = D == 64 ? 4 : 3;
+  static constexpr int kSmemQ = 0;
+  static constexpr int kSmemK = 2 * kTile;
+  static constexpr int kSmemV = kSmemK + kKStages * kTile;
+  static constexpr int kSmem = kSmemV + kVStages * kTile + 1024;
+};
+
+constexpr int kWg = 128;
+constexpr int kThreads = 3 * kWg;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kVLoadWarp = 10;
+constexpr int kSoftmaxRegs = 200, kControlRegs = 96;  // setmaxnreg split
+constexpr int kSplitRegs = 2 * kWg * kSoftmaxRegs + kWg * kControlRegs;
+static_assert(kSplitRegs <= kThreads * 168, "the register split exceeds the launch allocation");
+constexpr int kSched = 4;  // slots of the item queue
+constexpr int kTakers = 2 * kWg / 32 + 2;
+
+struct Bars {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t drain;
+  uint64_t sched_full[kSched], sched_empty[kSched];
+};
+
+struct Item {
+  int chunk, kh, tok0, tok_end;  // tokens [tok0, tok_end) are the sequence's (prefix: the batch's) from the first tile on
+  int qpos0;                     // chunk: own position of token tok0
+  int k_lo, k_valid;             // first key; keys of the table that hold data
+  int k_end;                     // prefix: end of the key range
+  int n0, n1, n;                 // K/V tiles of query tile 0, 1, and their maximum
+  const int32_t* table;
+  int64_t slab;
+};
+
+__device__ __forceinline__ Item decode_item(const SharedPrefixArgs& a, int64_t it, int64_t prefix_items) {
+  Item m{};
+  const int KV = a.p.kv_num_heads, TQ = a.tile_tokens;
+  if (it < prefix_items) {  // ((range, kv head), pair): neighbours share their K/V tiles in L2
+    const int pair = (int)(it % a.query_pairs);
+    const int64_t r = it / a.query_pairs;
+    m.kh = (int)(r % KV);
+    m.slab = r / KV;
+    m.tok0 = pair * 2 * TQ;
+    m.tok_end = a.p.num_tokens;
+    m.k_lo = (int)m.slab * a.split_tiles * kBN;
+    m.k_valid = a.p.prefix_length;
+    m.k_end = min(m.k_valid, m.k_lo + a.split_tiles * kBN);
+    m.n0 = (m.k_end - m.k_lo + kBN - 1) / kBN;
+    m.n1 = m.tok0 + TQ < m.tok_end ? m.n0 : 0;
+    m.n = m.n0;
+    m.table = a.p.prefix_block_table;
+    return m;
+  }
+  it -= prefix_items;
+  const int64_t pairs = __ldcg(a.seq_pairs + a.p.batch);
+  const int64_t pair_global = pairs - 1 - it / KV;  // later tiles, which see more keys, first
+  m.chunk = 1;
+  m.kh = (int)(it % KV);
+  int lo = 0, hi = a.p.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldcg(a.seq_pairs + mid) <= pair_global) lo = mid; else hi = mid - 1;
+  }
+  const int q0 = (int)(pair_global - __ldcg(a.seq_pairs + lo)) * 2 * TQ;
+  const int c0 = a.p.cumulative_sequence_length[lo], c1 = a.p.cumulative_sequence_length[lo + 1];
+  const int past = a.p.past_seqlens[lo];
+  m.tok0 = c0 + q0;
+  m.tok_end = c1;
+  m.qpos0 = past + q0;
+  m.k_valid = past + c1 - c0;
+  m.k_end = m.k_valid;
+  const int t1 = c1 - m.tok0;  // tokens from this pair on
+  m.n0 = (m.qpos0 + min(TQ, t1) + kBN - 1) / kBN;
+  m.n1 = t1 > TQ ? (m.qpos0 + min(2 * TQ, t1) + kBN - 1) / kBN : 0;
+  m.n = max(m.n0, m.n1);
+  m.table = a.p.block_table + (int64_t)lo * a.p.max_blocks_per_seq;
+  m.slab = a.splits;
+  return m;
+}
+
+__device__ __forceinline__ int tiles_of(const Item& m, int w) { return w ? m.n1 : m.n0; }
+
+// Page `page` of a V stage by plain loads: rows [0, rows) from block `blk` (position pos0 on), zeros
+// below, in the TMA's swizzle; then ordered before the tensor core's reads.
+template <int D>
+__device__ __noinline__ void fill_tail_page(uint8_t* stage, const B200SharedPrefixParams& p, int32_t blk, int pos0, int kh,
+                                            int page, int rows, int lane) {
+  const bool ok = blk >= 0 && blk < p.num_blocks;
+  const int64_t slot0 = (int64_t)blk * p.block_size + pos0 % p.block_size;
+  for (int i = lane; i < kPage * (D / 8); i += 32) {
+    const int r = i / (D / 8), box = (i % (D / 8)) >> 3, piece = i & 7;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < rows && ok)
+      v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.value_cache) +
+                                          (((slot0 + r) * p.kv_num_heads + kh) * D + box * 64) * 2 + piece * 16);
+    const int row = page * kPage + r;
+    *reinterpret_cast<uint4*>(stage + box * kBoxBytes + row * 128 + ((piece ^ (row & 7)) * 16)) = v;
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __grid_constant__ SharedPrefixArgs a,
+                                                                        const __grid_constant__ SharedPrefixMaps maps) {
+  using L = TcLayout<D>;
+  using MMA = mma_op<T>;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kIdQK = tc::idesc_f16(kBM, kBN, kBF16, false, false);
+  constexpr uint32_t kIdPV = tc::idesc_f16(kBM, D, kBF16, false, true);
+  constexpr int kKStages = L::kKStages, kVStages = L::kVStages;
+
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ __align__(8) Bars bars;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int s_failed;
+  __shared__ volatile long long s_item[kSched];
+
+  const B200SharedPrefixParams& p = a.p;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = a.group, H = p.num_heads, TQ = a.tile_tokens;
+
+  if (warp == kMmaWarp) tc::alloc(&tmem_slot, 512);
+  if (tid == 0) {
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&bars.q_full[w], 1);
+      mbar_init(&bars.q_empty[w], 1);
+      mbar_init(&bars.s_full[w], 1);
+      mbar_init(&bars.p_full[w], kWg);
+      mbar_init(&bars.o_done[w], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.v_empty[i], 1);
+    }
+    mbar_init(&bars.drain, 1);
+    for (int i = 0; i < kSched; ++i) {
+      mbar_init(&bars.sched_full[i], 1);
+      mbar_init(&bars.sched_empty[i], kTakers);
+    }
+    fence_mbar_init();
+    s_failed = 0;
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  wait_previous();       // the plan
+  release_dependents();  // the own kernel needs the plan, not this kernel
+  const int64_t prefix_items = (int64_t)a.splits * p.kv_num_heads * a.query_pairs;
+  const int64_t n_items = prefix_items + (int64_t)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads;
+
+  auto wait_idx = [&](uint64_t* bar, uint32_t index) -> bool {  // completion `index` of a barrier
+    if (s_failed) return false;
+    if (mbar_wait(bar, index & 1u)) return true;
+    set_status(p.device_status, kStatusTimeout);
+    s_failed = 1;
+    return false;
+  };
+  auto wait_warp = [&](uint64_t* bar, uint32_t index) -> bool { return __all_sync(0xffffffffu, wait_idx(bar, index)); };
+  auto failed_warp = [&]() -> bool { return __any_sync(0xffffffffu, s_failed != 0); };
+  auto drain_idx = [&](uint64_t* bar, uint32_t index) { mbar_wait(bar, index & 1u); };
+  auto fetch_item = [&](uint32_t k, int64_t& it) -> bool {
+    const uint32_t slot = k % kSched;
+    if (k >= (uint32_t)kSched && !wait_warp(&bars.sched_empty[slot], k / kSched - 1)) return false;
+    long long v = 0;
+    if (lane == 0) {
+      v = (long long)atomicAdd(a.next_item, 1ull);
+      s_item[slot] = v;
+      mbar_arrive(&bars.sched_full[slot]);
+    }
+    it = __shfl_sync(0xffffffffu, v, 0);
+    return true;
+  };
+  auto take_item = [&](uint32_t k, int64_t& it) -> bool {
+    const uint32_t slot = k % kSched;
+    if (!wait_warp(&bars.sched_full[slot], k / kSched)) return false;
+    it = s_item[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.sched_empty[slot]);
+    return true;
+  };
+
+  if (warp >= 2 * (kWg / 32)) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    if (warp == kLoadWarp || warp == kVLoadWarp) {
+      // ---------------------------------------------------------------- TMA producers
+      const bool is_v = warp == kVLoadWarp;
+      const uint32_t stages = is_v ? kVStages : kKStages;
+      uint64_t* full_bar = is_v ? bars.v_full : bars.k_full;
+      uint64_t* empty_bar = is_v ? bars.v_empty : bars.k_empty;
+      const CUtensorMap* map = is_v ? &maps.v_map : &maps.k_map;
+      const uint32_t ring = is_v ? L::kSmemV : L::kSmemK;
+      const uint32_t q_bytes = (uint32_t)(g * TQ * 128 * L::kBoxes);
+      uint32_t qc0 = 0, qc1 = 0, c = 0;
+      const int oob_z = p.num_blocks * p.block_size;  // past the cache: zero fill
+      const int page = (lane % (8 * L::kBoxes)) / L::kBoxes, half = lane % L::kBoxes;
+      const bool loader = lane < 8 * L::kBoxes;
+      bool ok = true;
+      for (uint32_t k = 0; ok && !failed_warp(); ++k) {
+        int64_t it;
+        if (!(ok = is_v ? take_item(k, it) : fetch_item(k, it)) || it >= n_items) break;
+        const Item m = decode_item(a, it, prefix_items);
+        if (!is_v) {
+          for (int w = 0; w < 2 && ok; ++w) {
+            if (tiles_of(m, w) == 0) continue;
+            const uint32_t qc = w ? qc1 : qc0;
+            if (qc > 0 && !(ok = wait_warp(&bars.q_empty[w], qc - 1))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&bars.q_full[w], q_bytes);
+            __syncwarp();
+            if (lane < L::kBoxes)
+              tma_load_3d(smem + L::kSmemQ + w * L::kTile + lane * kBoxBytes, &maps.q_map, &bars.q_full[w], lane * 64,
+                          m.kh * g, m.tok0 + w * TQ);
+            if (w) qc1 = qc + 1; else qc0 = qc + 1;
+          }
+        }
+        auto block_of = [&](int j) -> int32_t {
+          const int pos = m.k_lo + j * kBN + page * kPage;
+          return loader && pos < m.k_valid ? __ldg(m.table + pos / p.block_size) : -1;
+        };
+        int32_t blk_next = block_of(0);
+        for (int j = 0; j < m.n && ok; ++j) {
+          const int pos0 = m.k_lo + j * kBN + page * kPage;
+          const int32_t blk = blk_next;
+          if (j + 1 < m.n) blk_next = block_of(j + 1);  // in flight during the stage wait below
+          const bool blk_ok = blk >= 0 && blk < p.num_blocks;
+          if (!is_v && loader && pos0 < m.k_valid && !blk_ok) set_status(p.device_status, kStatusBadBlock);
+          const int z = blk_ok ? blk * p.block_size + pos0 % p.block_size : oob_z;
+          const uint32_t st = c % stages;
+          if (c >= stages && !(ok = wait_warp(&empty_bar[st], c / stages - 1))) break;
+          // The V page that reaches past the last key: its rows by plain loads, its unused slots zeroed
+          // (whatever they hold, NaN included, must not meet P = 0 in the MMA).
+          const int valid = min(kBN, m.k_valid - (m.k_lo + j * kBN));
+          const int rows = is_v ? valid & (kPage - 1) : 0;
+          const int tail_page = valid >> 4;
+          if (rows) {
+            const int32_t tblk = __shfl_sync(0xffffffffu, blk, L::kBoxes * tail_page);
+            const int tpos = __shfl_sync(0xffffffffu, pos0, L::kBoxes * tail_page);
+            fill_tail_page<D>(smem + ring + st * L::kTile, p, tblk, tpos, m.kh, tail_page, rows, lane);
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], rows ? L::kTile - kPage * 128 * L::kBoxes : L::kTile);
+          __syncwarp();
+          if (loader && !(rows && page == tail_page))
+            tma_load_3d(smem + ring + st * L::kTile + half * kBoxBytes + page * (kPage * 128), map, &full_bar[st],
+                        half * 64, m.kh, z);
+          ++c;
+        }
+      }
+      if (qc0 > 0) drain_idx(&bars.q_full[0], qc0 - 1);
+      if (qc1 > 0) drain_idx(&bars.q_full[1], qc1 - 1);
+      for (uint32_t i = (c > stages ? c - stages : 0); i < c; ++i) drain_idx(&full_bar[i % stages], i / stages);
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------------- MMA issuer
+      const bool leader = tc::elect_one();
+      uint32_t qc0 = 0, qc1 = 0, pc0 = 0, pc1 = 0, kvc = 0;
+      bool issued = false, ok = true;
+      for (uint32_t k = 0; ok && !failed_warp(); ++k) {
+        int64_t it;
+        if (!(ok = take_item(k, it)) || it >= n_items) break;
+        const Item m = decode_item(a, it, prefix_items);
+#pragma unroll 1
+        for (int j = 0; j <= m.n && ok; ++j) {
+          const uint32_t ki = kvc + j, vi = ki - 1;
+          if (j > 0 && !(ok = wait_warp(&bars.v_full[vi % kVStages], vi / kVStages))) break;
+          bool k_ready = false;
+#pragma unroll 1
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t pc = w ? pc1 : pc0;
+            const int nw = tiles_of(m, w);
+            if (j > 0 && j - 1 < nw) {  // O_w (+)= P_w(j-1) V_(j-1)
+              if (!(ok = wait_warp(&bars.p_full[w], pc))) break;
+              tc::fence_after_sync();
+              const uint32_t pbuf = tmem + w * 128, obuf = tmem + 256 + w * 128;
+              const uint64_t vdesc0 = tc::smem_desc(sbase + L::kSmemV + (vi % kVStages) * L::kTile, kBoxBytes, 1024);
+#pragma unroll
+              for (int kk = 0; kk < kBN / 16; ++kk) {
+                const uint64_t vdesc = vdesc0 + (uint64_t)(kk * (2048 >> 4));
+                const uint32_t pcol = pbuf + (kk >> 1) * 32 + (kk & 1) * 8;
+                if (leader) {
+                  tc::mma_ts(obuf, pcol, vdesc, kIdPV, (j > 1 || kk > 0) ? 1u : 0u);
+                  if (kBF16) tc::mma_ts(obuf, pcol + 16, vdesc, kIdPV, 1u);
+                }
+              }
+              if (leader && j == nw) tc::commit(&bars.o_done[w]);
+              if (w) pc1 = pc + 1; else pc0 = pc + 1;
+            }
+            if (j < nw) {  // S_w(j) = Q_w K_j^T
+              if (!k_ready) {
+                if (!(ok = wait_warp(&bars.k_full[ki % kKStages], ki / kKStages))) break;
+                k_ready = true;
+              }
+              if (j == 0 && !(ok = wait_warp(&bars.q_full[w], w ? qc1 : qc0))) break;
+              const uint64_t kdesc0 = tc::smem_desc(sbase + L::kSmemK + (ki % kKStages) * L::kTile, 16, 1024);
+              const uint64_t qdesc0 = tc::smem_desc(sbase + L::kSmemQ + w * L::kTile, 16, 1024);
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = (kk >> 2) * kBoxBytes + (kk & 3) * 32;
+                const uint64_t qdesc = qdesc0 + (uint64_t)(off >> 4), kdesc = kdesc0 + (uint64_t)(off >> 4);
+                if (leader) tc::mma_ss(tmem + w * 128, qdesc, kdesc, kIdQK, kk > 0);
+              }
+              if (leader) tc::commit(&bars.s_full[w]);
+              if (j == nw - 1) {
+                if (leader) tc::commit(&bars.q_empty[w]);
+                if (w) ++qc1; else ++qc0;
+              }
+              issued = true;
+            }
+          }
+          if (!ok) break;
+          if (leader && j > 0) tc::commit(&bars.v_empty[vi % kVStages]);
+          if (leader && k_ready) tc::commit(&bars.k_empty[ki % kKStages]);
+        }
+        kvc += m.n;
+      }
+      if (issued) {
+        if (leader) tc::commit(&bars.drain);
+        drain_idx(&bars.drain, 0);
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------------------------ softmax + epilogue
+    const int w = warp >> 2, row = tid & (kWg - 1);
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t sbuf = tmem + w * 128 + lane_off, obuf = tmem + 256 + w * 128 + lane_off;
+    const float qk_scale = p.softcap > 0.f ? p.scale : p.scale * kLog2e;
+    const int tl = row / g, hl = row % g;
+    uint32_t t = 0, items = 0;
+    for (uint32_t k = 0; !failed_warp(); ++k) {
+      int64_t it;
+      if (!take_item(k, it) || it >= n_items) break;
+      const Item m = decode_item(a, it, prefix_items);
+      const int nw = tiles_of(m, w);
+      if (nw == 0) continue;
+      const int tok = m.tok0 + w * TQ + tl;
+      const bool row_ok = tl < TQ && tok < m.tok_end;
+      // last key the row sees; rows without a token see everything (their results are dropped)
+      const int last = m.chunk && row_ok ? m.qpos0 + w * TQ + tl : m.k_end - 1;
+      float m_run = -INFINITY, l_run = 0.f;
+      bool ok = true;
+      for (int j = 0; j < nw; ++j, ++t) {
+        if (!(ok = wait_warp(&bars.s_full[w], t))) break;
+        tc::fence_after_sync();
+        const int kbase = m.k_lo + j * kBN;
+        // Unmasked tiles keep raw scores, the scale goes into the exponent's FMA; others are rewritten
+        // in place as scaled log2 values.  Warp-uniform.
+        const bool raw = __all_sync(0xffffffffu, kbase + kBN - 1 <= last) && p.softcap <= 0.f && qk_scale > 0.f;
+        float mx[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx[r] = -INFINITY;
+        if (raw) {
+          float sv[kBN / 32][32];
+#pragma unroll
+          for (int c = 0; c < kBN / 32; ++c) tc::ld32(sbuf + c * 32, sv[c]);
+          tc::wait_ld();
+#pragma unroll
+          for (int c = 0; c < kBN / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx[i & 3] = tc::max3(mx[i & 3], sv[c][2 * i], sv[c][2 * i + 1]);
+        } else {
+          const int vhi = last - kbase;
+#pragma unroll 1
+          for (int c = 0; c < kBN / 32; ++c) {
+            float x[32];
+            tc::ld32(sbuf + c * 32, x);
+            tc::wait_ld();
+            if (p.softcap > 0.f) {
+              // cap tanh(y / cap), tanh(u) = 1 - 2 / (1 + e^(2u))
+              const float two_log2e_over_cap = 2.f * kLog2e / p.softcap, cap_log2e = p.softcap * kLog2e;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float e = tc::ex2(fminf(x[i] * qk_scale * two_log2e_over_cap, 126.f));
+                x[i] = cap_log2e * (1.f - __fdividef(2.f, 1.f + e));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] *= qk_scale;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = c * 32 + i <= vhi ? x[i] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx[i & 3] = tc::max3(mx[i & 3], x[2 * i], x[2 * i + 1]);
+            tc::st32(sbuf + c * 32, x);
+          }
+          tc::wait_st();
+        }
+        float m_tile = tc::max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+        if (raw) m_tile *= qk_scale;
+        const float m_new = fmaxf(m_run, m_tile);
+        const bool grow = m_new > m_run + 8.0f;
+        const float alpha = (grow && m_run != -INFINITY) ? tc::ex2(m_run - m_new) : 1.0f;
+        if (grow) {
+          l_run *= (m_run == -INFINITY ? 0.f : alpha);
+          m_run = m_new;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, grow && alpha != 1.0f)) {
+          // s_full of tile j also says that P V of tile j - 1 has landed in O
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            float r[16];
+            tc::ld16(obuf + c * 16, r);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] *= alpha;
+            tc::st16(obuf + c * 16, r);
+          }
+          tc::wait_st();
+        }
+        // P = 2^(x - mu) per 32-column chunk over the chunk's first 16 columns (bf16: lo halves over
+        // the last 16); each chunk is read before it is overwritten
+        const float mu = m_run == -INFINITY ? 0.f : m_run;
+        const float kscale = raw ? qk_scale : 1.0f;
+        const float2 ks2 = make_float2(kscale, kscale), nmu2 = make_float2(-mu, -mu);
+        float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto exp_chunk = [&](const float(&x)[32], int c) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 e = tc::fma2(make_float2(x[2 * i], x[2 * i + 1]), ks2, nmu2);
+            const float2 pr = i % kPolyEvery == kPolyEvery - 1 ? tc::exp2_poly2(e) : make_float2(tc::ex2(e.x), tc::ex2(e.y));
+            ls[i & 1] = tc::add2(ls[i & 1], pr);
+            if constexpr (kBF16) {
+              // hi: the upper 16 bits; lo: the exact rest, rounded
+              const uint32_t u0 = __float_as_uint(pr.x), u1 = __float_as_uint(pr.y);
+              hi[i] = __byte_perm(u0, u1, 0x7632);
+              const float2 r = tc::sub2(pr, make_float2(__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)));
+              lo[i] = MMA::pack(r.x, r.y);
+            } else {
+              hi[i] = MMA::pack(pr.x, pr.y);
+            }
+          }
+          tc::st16u(sbuf + c * 32, hi);
+          if constexpr (kBF16) tc::st16u(sbuf + c * 32 + 16, lo);
+        };
+        float xa[32], xb[32];
+        tc::ld32(sbuf, xa);
+        tc::wait_ld();
+#pragma unroll 1
+        for (int c = 0; c < kBN / 32; c += 2) {
+          tc::ld32(sbuf + (c + 1) * 32, xb);
+          exp_chunk(xa, c);
+          tc::wait_ld();
+          if (c + 2 < kBN / 32) tc::ld32(sbuf + (c + 2) * 32, xa);
+          exp_chunk(xb, c + 1);
+          tc::wait_ld();
+        }
+        l_run += (ls[0].x + ls[1].x) + (ls[0].y + ls[1].y);
+        tc::wait_st();
+        tc::fence_before_sync();
+        mbar_arrive(&bars.p_full[w]);
+      }
+      if (!ok) break;
+      if (!wait_warp(&bars.o_done[w], items++)) break;
+      tc::fence_after_sync();
+      const int64_t at = m.slab * a.rows + (int64_t)tok * H + m.kh * g + hl;
+      if (row_ok) a.slab_ml[at] = make_float2(m_run, l_run);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        tc::ld32(obuf + c * 32, o);
+        tc::wait_ld();
+        if (row_ok) {
+          float4* dst = reinterpret_cast<float4*>(a.slab_o + at * D + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      tc::fence_before_sync();
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (warp == kMmaWarp) tc::dealloc(tmem, 512);
+}
+
+template <typename T, int D>
+cudaError_t launch_tc_t(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms, cudaStream_t stream) {
+  auto kernel = shared_prefix_tc_kernel<T, D>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  static std::atomic<uint32_t> ready[64];  // per device: attributes set and checked
+  if (!ready[dev & 63].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    cudaFuncAttributes attr;  // setmaxnreg.inc waits until the launch allocation covers the split
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs * kThreads < kSplitRegs) return cudaErrorInvalidConfiguration;
+    ready[dev & 63].store(1, std::memory_order_release);
+  }
+  return launch_dependent(kernel, dim3(num_sms), dim3(kThreads), TcLayout<D>::kSmem, stream, a, maps);
+}
+
+}  // namespace
+
+cudaError_t launch_shared_prefix_tc(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms,
+                                    cudaStream_t stream) {
+  const bool bf = a.p.act_dtype == B200_DTYPE_BFLOAT16;
+  if (a.p.head_size == 64)
+    return bf ? launch_tc_t<__nv_bfloat16, 64>(a, maps, num_sms, stream) : launch_tc_t<__half, 64>(a, maps, num_sms, stream);
+  return bf ? launch_tc_t<__nv_bfloat16, 128>(a, maps, num_sms, stream) : launch_tc_t<__half, 128>(a, maps, num_sms, stream);
+}
+
+}  // namespace b200

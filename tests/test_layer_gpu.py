@@ -588,6 +588,9 @@ def test_prefix_refusals():
                    dict(H=6), dict(table=c["table"].t()), dict(sink=c["q"][0])):
         with pytest.raises((B200Error, ZeroDivisionError)):
             prefix_call({**c, **change})
+    with pytest.raises(B200Error, match="workspace"):
+        big = prefix_case(6, [20], [1], 100, 8, 2, 128)
+        prefix_call(big, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
 
 
 def test_layer_in_a_graph():
