@@ -5,6 +5,15 @@
 //   position[axis of the pair] of the tables
 //
 // Memory bound: every query, key and value row is read once and written once.
+//
+// rotary_append_vec_kernel: a thread owns a unit of 16 channels (two 16-byte pieces: the two halves
+// of 8 rotary pairs, or 16 channels that do not turn) and walks the token's heads with it, so the 8
+// cos and sin values are loaded once per token and stay in registers; all heads' loads go out
+// before the first is needed.  rotary_append_kernel takes what is not aligned to such units.
+//
+// Of several tokens with one slot the last is stored.  Up to B200_ROTARY_APPEND_SCAN_TOKENS tokens,
+// a CTA compares its tokens' slots with every later one (kScanTokens tokens per CTA share the reads of
+// the list); beyond, where that work grows with the square, a hash table is filled first.
 #include <algorithm>
 
 #include "b200_common.cuh"
@@ -148,6 +157,270 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(const B200RotaryAppe
   for (int i = tid; i < KV * d; i += threads) store_cached<T>(p, false, slot, i / d, i % d, act<T>::to_f(v[i]));
 }
 
+// Whether a later token names the same slot, for the TOKENS tokens from t0 on (bit i: token t0 + i).
+template <int TOKENS>
+__device__ __forceinline__ int later_same_slot(const B200RotaryAppendParams& p, int64_t t0, const int32_t (&slot)[TOKENS]) {
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int32_t* list = p.slot_mapping;
+  const int64_t n = p.num_tokens, from = t0 + TOKENS;
+  int later = 0;
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i)
+#pragma unroll
+    for (int j = i + 1; j < TOKENS; ++j) later |= (slot[i] == slot[j]) << i;
+  auto compare = [&](int32_t other) {
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) later |= (slot[i] == other) << i;
+  };
+  // up to the next 16-byte boundary, whole vectors, the rest
+  const int64_t head = min(n - from, (int64_t)(-(reinterpret_cast<uintptr_t>(list + from) >> 2) & 3));
+  if (tid < head) compare(__ldg(list + from + tid));
+  const int64_t vecs = from < n ? (n - from - head) / 4 : 0;
+  const int4* wide = reinterpret_cast<const int4*>(list + from + (head > 0 ? head : 0));
+#pragma unroll 4
+  for (int64_t v = tid; v < vecs; v += threads) {
+    const int4 w = __ldg(wide + v);
+    compare(w.x);
+    compare(w.y);
+    compare(w.z);
+    compare(w.w);
+  }
+  for (int64_t u = from + head + vecs * 4 + tid; u < n; u += threads) compare(__ldg(list + u));
+  int any = 0;
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) any |= (__syncthreads_or(later >> i & 1) ? 1 : 0) << i;
+  return any;
+}
+
+// 8 table values as fp32.
+template <typename T>
+__device__ __forceinline__ void load_table8(const B200RotaryAppendParams& p, const void* table, int64_t at, float (&v)[8]) {
+  if (p.table_dtype == B200_DTYPE_FLOAT) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(table) + at));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(table) + at) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(table) + at));
+    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = mma_op<T>::unpack(r[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
+  const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = mma_op<T>::unpack(r[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(mma_op<T>::pack(v[0], v[1]), mma_op<T>::pack(v[2], v[3]), mma_op<T>::pack(v[4], v[5]),
+                    mma_op<T>::pack(v[6], v[7]));
+}
+
+// 8 e4m3 codes of v / scale, saturating (IEEE division: the bytes b200_kv_append writes).
+__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float scale) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(
+        make_float2(__fdiv_rn(v[4 * i], scale), __fdiv_rn(v[4 * i + 1], scale)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(
+        make_float2(__fdiv_rn(v[4 * i + 2], scale), __fdiv_rn(v[4 * i + 3], scale)), __NV_SATFINITE, __NV_E4M3);
+    w[i] = lo | (hi << 16);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+constexpr int kVecThreads = 128;
+constexpr int kScanTokens = 4;
+constexpr int kHeadsInFlight = 4;  // heads whose 32 bytes a thread has in flight
+
+// CTA: TOKENS tokens x heads [blockIdx.y * cta_heads, + cta_heads) of the query, key and value heads in
+// that order; thread (unit of `units`, head offset of `head_step`).
+template <typename T, bool FP8, int TOKENS>
+__global__ void __launch_bounds__(kVecThreads) rotary_append_vec_kernel(const __grid_constant__ B200RotaryAppendParams p,
+                                                                         const int* keys, const int* last,
+                                                                         uint32_t capacity, int units, int head_step,
+                                                                         int cta_heads) {
+  const int64_t t0 = (int64_t)blockIdx.x * TOKENS;
+  const int tid = threadIdx.x, unit = tid % units, hb = tid / units;
+  const int d = p.head_size, H = p.num_heads, KV = p.kv_num_heads, half = p.rotary_dim / 2;
+  const int h_begin = blockIdx.y * cta_heads, h_end = min(H + 2 * KV, h_begin + cta_heads);
+  const bool turns = unit < p.rotary_dim / 16;
+  // first channels of the unit's two pieces in query and key heads
+  int ca, cb;
+  if (turns) {
+    ca = p.rotary_offset + (p.rotary_interleaved ? 16 * unit : 8 * unit);
+    cb = p.rotary_interleaved ? ca + 8 : ca + half;
+  } else {
+    ca = 16 * (unit - p.rotary_dim / 16);
+    cb = ca + 8;
+    ca += ca < p.rotary_offset ? 0 : p.rotary_dim;
+    cb += cb < p.rotary_offset ? 0 : p.rotary_dim;
+  }
+  int32_t slot[TOKENS];
+  int store = 0;
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) slot[i] = t0 + i < p.num_tokens ? __ldg(p.slot_mapping + t0 + i) : -1;
+  if (h_end > H) {  // this CTA has rows to store
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) {
+      const bool valid = slot[i] >= -1 && (int64_t)slot[i] < (int64_t)p.num_blocks * p.block_size;
+      if (!valid && tid == 0) set_status(p.device_status, kStatusBadSlot);
+      store |= (valid && slot[i] >= 0) << i;
+    }
+    if (keys) {
+#pragma unroll
+      for (int i = 0; i < TOKENS; ++i)
+        if (store >> i & 1) store &= ~((last_token(slot[i], (int)(t0 + i), keys, last, capacity) != (int)(t0 + i)) << i);
+    } else {
+      store &= ~later_same_slot<TOKENS>(p, t0, slot);
+    }
+  }
+#pragma unroll 1
+  for (int i = 0; i < TOKENS; ++i) {
+    const int64_t t = t0 + i;
+    if (t >= p.num_tokens) break;
+    const int32_t sl = slot[i];
+    const bool keep = store >> i & 1;
+    float c[8], s[8];
+    bool have = false;
+    for (int h0 = h_begin + hb; h0 < h_end; h0 += kHeadsInFlight * head_step) {
+      uint4 xa[kHeadsInFlight], xb[kHeadsInFlight];
+#pragma unroll
+      for (int k = 0; k < kHeadsInFlight; ++k) {
+        const int h = h0 + k * head_step;
+        if (h >= h_end || (h >= H && !keep)) continue;
+        const T* row = h < H ? static_cast<const T*>(p.query) + t * p.query_row_stride + (int64_t)h * d
+                     : h < H + KV ? static_cast<const T*>(p.key) + t * p.key_row_stride + (int64_t)(h - H) * d
+                                  : static_cast<const T*>(p.value) + t * p.value_row_stride + (int64_t)(h - H - KV) * d;
+        const bool value = h >= H + KV;
+        xa[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit : ca));
+        xb[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit + 8 : cb));
+      }
+      if (turns && !have && h0 < H + KV) {
+        have = true;
+        const int pair = 8 * unit, axis = axis_of(p, pair);
+        if (axis_of(p, pair + 7) == axis) {
+          const int64_t pos = position_of(p, axis, t);
+          if (pos >= 0 && pos < p.rotary_positions) {
+            load_table8<T>(p, p.cos_cache, pos * half + pair, c);
+            load_table8<T>(p, p.sin_cache, pos * half + pair, s);
+          } else {
+            set_status(p.device_status, kStatusBadPosition);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              c[j] = 1.f;
+              s[j] = 0.f;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int64_t pos = position_of(p, axis_of(p, pair + j), t);
+            const bool in = pos >= 0 && pos < p.rotary_positions;
+            if (!in) set_status(p.device_status, kStatusBadPosition);
+            c[j] = in ? table_value<T>(p, p.cos_cache, pos * half + pair + j) : 1.f;
+            s[j] = in ? table_value<T>(p, p.sin_cache, pos * half + pair + j) : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kHeadsInFlight; ++k) {
+        const int h = h0 + k * head_step;
+        if (h >= h_end || (h >= H && !keep)) continue;
+        const bool value = h >= H + KV;
+        float a[8], b[8];
+        unpack8<T>(xa[k], a);
+        unpack8<T>(xb[k], b);
+        if (turns && !value) {
+          if (p.rotary_interleaved) {  // pairs (0,1), (2,3), .. of the 16 contiguous channels
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float y0 = a[2 * j] * c[j] - a[2 * j + 1] * s[j], y1 = a[2 * j + 1] * c[j] + a[2 * j] * s[j];
+              a[2 * j] = y0;
+              a[2 * j + 1] = y1;
+              const float z0 = b[2 * j] * c[4 + j] - b[2 * j + 1] * s[4 + j];
+              const float z1 = b[2 * j + 1] * c[4 + j] + b[2 * j] * s[4 + j];
+              b[2 * j] = z0;
+              b[2 * j + 1] = z1;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float y0 = a[j] * c[j] - b[j] * s[j], y1 = b[j] * c[j] + a[j] * s[j];
+              a[j] = y0;
+              b[j] = y1;
+            }
+          }
+          xa[k] = pack8<T>(a);
+          xb[k] = pack8<T>(b);
+        }
+        if (h < H) {
+          T* row = static_cast<T*>(p.output) + t * p.output_row_stride + (int64_t)h * d;
+          *reinterpret_cast<uint4*>(row + ca) = xa[k];
+          *reinterpret_cast<uint4*>(row + cb) = xb[k];
+          continue;
+        }
+        const int kh = value ? h - H - KV : h - H;
+        const int64_t at = ((int64_t)sl * KV + kh) * d;
+        void* cache = value ? p.value_cache : p.key_cache;
+        const int sa = value ? 16 * unit : ca, sb = value ? 16 * unit + 8 : cb;
+        if constexpr (FP8) {
+          const float scale = __ldg((value ? p.v_scale : p.k_scale) + (int64_t)(sl / p.block_size) * KV + kh);
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sa) = e4m3x8(a, scale);
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sb) = e4m3x8(b, scale);
+        } else {
+          *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sa) = xa[k];
+          *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sb) = xb[k];
+        }
+      }
+    }
+  }
+}
+
+// Whether every head splits into 16-byte pieces as the vector kernel reads and writes them.
+bool vector_form(const B200RotaryAppendParams& p) {
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.key) |
+                          reinterpret_cast<uintptr_t>(p.value) | reinterpret_cast<uintptr_t>(p.output) |
+                          reinterpret_cast<uintptr_t>(p.key_cache) | reinterpret_cast<uintptr_t>(p.value_cache) |
+                          reinterpret_cast<uintptr_t>(p.cos_cache) | reinterpret_cast<uintptr_t>(p.sin_cache);
+  const int64_t strides = p.query_row_stride | p.key_row_stride | p.value_row_stride | p.output_row_stride;
+  return bases % 16 == 0 && strides % 8 == 0 && p.head_size % 16 == 0 && p.head_size / 16 <= kVecThreads &&
+         p.rotary_dim % 16 == 0 && p.rotary_offset % 8 == 0;
+}
+
+template <typename T, bool FP8>
+void launch_vec(const B200RotaryAppendParams& p, const int* keys, const int* last, uint32_t cap, int num_sms,
+                cudaStream_t stream) {
+  const int units = p.head_size / 16, head_step = kVecThreads / units, heads = p.num_heads + 2 * p.kv_num_heads;
+  const int per_pass = head_step;
+  // Few tokens: heads spread over CTAs, one per thread, for the shortest chain of loads.
+  const int64_t one_pass = (int64_t)p.num_tokens * ((heads + per_pass - 1) / per_pass);
+  const bool spread = one_pass <= 8 * (int64_t)num_sms;
+  const int cta_heads = spread ? per_pass : heads;
+  const unsigned splits = (unsigned)((heads + cta_heads - 1) / cta_heads);
+  const int threads = units * head_step;
+  if (p.num_tokens < 16 * num_sms)
+    rotary_append_vec_kernel<T, FP8, 1><<<dim3(p.num_tokens, splits), threads, 0, stream>>>(p, keys, last, cap, units,
+                                                                                           head_step, cta_heads);
+  else
+    rotary_append_vec_kernel<T, FP8, kScanTokens><<<dim3((p.num_tokens + kScanTokens - 1) / kScanTokens, splits), threads,
+                                                    0, stream>>>(p, keys, last, cap, units, head_step, cta_heads);
+}
+
 uint32_t table_capacity(int tokens) {
   uint32_t cap = 64;
   while (cap < 2 * (uint32_t)tokens) cap <<= 1;
@@ -160,7 +433,7 @@ size_t rotary_append_workspace(const B200RotaryAppendParams& p) {
   return p.num_tokens > B200_ROTARY_APPEND_SCAN_TOKENS ? 2 * sizeof(int) * (size_t)table_capacity(p.num_tokens) : 0;
 }
 
-cudaError_t launch_rotary_append(const B200RotaryAppendParams& p, int, cudaStream_t stream) {
+cudaError_t launch_rotary_append(const B200RotaryAppendParams& p, int num_sms, cudaStream_t stream) {
   int *keys = nullptr, *last = nullptr;
   uint32_t cap = 0;
   if (p.num_tokens > B200_ROTARY_APPEND_SCAN_TOKENS) {
@@ -173,7 +446,16 @@ cudaError_t launch_rotary_append(const B200RotaryAppendParams& p, int, cudaStrea
         p.slot_mapping, p.num_tokens, (int64_t)p.num_blocks * p.block_size, keys, last, cap);
     add_launches(2);
   }
-  if (p.act_dtype == B200_DTYPE_BFLOAT16)
+  const bool bf = p.act_dtype == B200_DTYPE_BFLOAT16;
+  if (vector_form(p)) {
+    if (p.cache_dtype == B200_DTYPE_FLOAT8E4M3FN) {
+      if (bf) launch_vec<__nv_bfloat16, true>(p, keys, last, cap, num_sms, stream);
+      else launch_vec<__half, true>(p, keys, last, cap, num_sms, stream);
+    } else {
+      if (bf) launch_vec<__nv_bfloat16, false>(p, keys, last, cap, num_sms, stream);
+      else launch_vec<__half, false>(p, keys, last, cap, num_sms, stream);
+    }
+  } else if (bf)
     rotary_append_kernel<__nv_bfloat16><<<p.num_tokens, 256, 0, stream>>>(p, keys, last, cap);
   else
     rotary_append_kernel<__half><<<p.num_tokens, 256, 0, stream>>>(p, keys, last, cap);
