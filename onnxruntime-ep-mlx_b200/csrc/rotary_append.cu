@@ -7,9 +7,9 @@
 // Memory bound: every query, key and value row is read once and written once.
 //
 // rotary_append_vec_kernel: a thread owns a unit of 16 channels (two 16-byte pieces: the two halves
-// of 8 rotary pairs, or 16 channels that do not turn) and walks the token's heads with it, so the 8
-// cos and sin values are loaded once per token and stay in registers; all heads' loads go out
-// before the first is needed.  rotary_append_kernel takes what is not aligned to such units.
+// of 8 rotary pairs, or 16 channels that do not turn) and walks the token's heads with it.  The cos and
+// sin values of a CTA's tokens, gathered once per pair (axes may change anywhere between pairs), wait in
+// shared memory and stay in registers over the heads.  rotary_append_kernel takes what is not aligned to such units.
 //
 // Of several tokens with one slot the last is stored.  Up to B200_ROTARY_APPEND_SCAN_TOKENS tokens,
 // a CTA compares its tokens' slots with every later one (kScanTokens tokens per CTA share the reads of
@@ -192,26 +192,6 @@ __device__ __forceinline__ int later_same_slot(const B200RotaryAppendParams& p, 
   return any;
 }
 
-// 8 table values as fp32.
-template <typename T>
-__device__ __forceinline__ void load_table8(const B200RotaryAppendParams& p, const void* table, int64_t at, float (&v)[8]) {
-  if (p.table_dtype == B200_DTYPE_FLOAT) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(table) + at));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(table) + at) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(table) + at));
-    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = mma_op<T>::unpack(r[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
   const uint32_t r[4] = {w.x, w.y, w.z, w.w};
@@ -245,41 +225,80 @@ __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float scale) {
 
 constexpr int kVecThreads = 128;
 constexpr int kScanTokens = 4;
-constexpr int kHeadsInFlight = 4;  // heads whose 32 bytes a thread has in flight
+
+// The cos and sin values of TOKENS tokens from t0 on into shared memory, [token][pair] each (1 and 0
+// where a position is out of range).
+template <typename T, int TOKENS>
+__device__ __forceinline__ void load_turns(const B200RotaryAppendParams& p, int64_t t0, int half, float* cos_s, float* sin_s) {
+  bool bad = false;
+  for (int j = threadIdx.x; j < TOKENS * half; j += blockDim.x) {
+    const int i = TOKENS == 1 ? 0 : j / half, pair = j - i * half;
+    if (t0 + i >= p.num_tokens) break;
+    const int64_t pos = position_of(p, p.axes == 1 ? 0 : axis_of(p, pair), t0 + i);
+    const bool in = pos >= 0 && pos < p.rotary_positions;
+    cos_s[j] = in ? table_value<T>(p, p.cos_cache, pos * half + pair) : 1.f;
+    sin_s[j] = in ? table_value<T>(p, p.sin_cache, pos * half + pair) : 0.f;
+    bad |= !in;
+  }
+  if (bad) set_status(p.device_status, kStatusBadPosition);
+}
+
+// Turn a unit: pairs (a[j], b[j]), or the neighbours of the 16 contiguous channels a, b.
+__device__ __forceinline__ void turn(bool interleaved, const float (&c)[8], const float (&s)[8], float (&a)[8], float (&b)[8]) {
+  auto pair = [](float& x0, float& x1, float co, float si) {
+    const float y0 = x0 * co - x1 * si;
+    x1 = x1 * co + x0 * si;
+    x0 = y0;
+  };
+  if (interleaved) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      pair(a[2 * j], a[2 * j + 1], c[j], s[j]);
+      pair(b[2 * j], b[2 * j + 1], c[4 + j], s[4 + j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pair(a[j], b[j], c[j], s[j]);
+  }
+}
 
 // CTA: TOKENS tokens x heads [blockIdx.y * cta_heads, + cta_heads) of the query, key and value heads in
 // that order; thread (unit of `units`, head offset of `head_step`).
 template <typename T, bool FP8, int TOKENS>
-__global__ void __launch_bounds__(kVecThreads) rotary_append_vec_kernel(const __grid_constant__ B200RotaryAppendParams p,
-                                                                         const int* keys, const int* last,
-                                                                         uint32_t capacity, int units, int head_step,
-                                                                         int cta_heads) {
+__global__ void __launch_bounds__(kVecThreads, 7) rotary_append_vec_kernel(const __grid_constant__ B200RotaryAppendParams p,
+                                                                            const int* keys, const int* last,
+                                                                            uint32_t capacity, int units, int head_step,
+                                                                            int cta_heads) {
   const int64_t t0 = (int64_t)blockIdx.x * TOKENS;
   const int tid = threadIdx.x, unit = tid % units, hb = tid / units;
   const int d = p.head_size, H = p.num_heads, KV = p.kv_num_heads, half = p.rotary_dim / 2;
-  const int h_begin = blockIdx.y * cta_heads, h_end = min(H + 2 * KV, h_begin + cta_heads);
-  const bool turns = unit < p.rotary_dim / 16;
+  const int h_first = blockIdx.y * cta_heads + hb, h_end = min(H + 2 * KV, (int)(blockIdx.y + 1) * cta_heads);
+  const int q_end = min(H, h_end);
+  const bool turns = unit < p.rotary_dim / 16, interleaved = p.rotary_interleaved != 0;
   // first channels of the unit's two pieces in query and key heads
   int ca, cb;
   if (turns) {
-    ca = p.rotary_offset + (p.rotary_interleaved ? 16 * unit : 8 * unit);
-    cb = p.rotary_interleaved ? ca + 8 : ca + half;
+    ca = p.rotary_offset + (interleaved ? 16 * unit : 8 * unit);
+    cb = interleaved ? ca + 8 : ca + half;
   } else {
     ca = 16 * (unit - p.rotary_dim / 16);
     cb = ca + 8;
     ca += ca < p.rotary_offset ? 0 : p.rotary_dim;
     cb += cb < p.rotary_offset ? 0 : p.rotary_dim;
   }
-  int32_t slot[TOKENS];
+  extern __shared__ float turns_s[];  // cos [TOKENS][half], sin [TOKENS][half]
+  __shared__ int32_t slots[TOKENS];
+  load_turns<T, TOKENS>(p, t0, half, turns_s, turns_s + TOKENS * half);
   int store = 0;
-#pragma unroll
-  for (int i = 0; i < TOKENS; ++i) slot[i] = t0 + i < p.num_tokens ? __ldg(p.slot_mapping + t0 + i) : -1;
   if (h_end > H) {  // this CTA has rows to store
+    int32_t slot[TOKENS];
 #pragma unroll
     for (int i = 0; i < TOKENS; ++i) {
+      slot[i] = t0 + i < p.num_tokens ? __ldg(p.slot_mapping + t0 + i) : -1;
       const bool valid = slot[i] >= -1 && (int64_t)slot[i] < (int64_t)p.num_blocks * p.block_size;
       if (!valid && tid == 0) set_status(p.device_status, kStatusBadSlot);
       store |= (valid && slot[i] >= 0) << i;
+      if (tid == 0) slots[i] = slot[i];
     }
     if (keys) {
 #pragma unroll
@@ -289,103 +308,68 @@ __global__ void __launch_bounds__(kVecThreads) rotary_append_vec_kernel(const __
       store &= ~later_same_slot<TOKENS>(p, t0, slot);
     }
   }
+  __syncthreads();
 #pragma unroll 1
   for (int i = 0; i < TOKENS; ++i) {
     const int64_t t = t0 + i;
     if (t >= p.num_tokens) break;
-    const int32_t sl = slot[i];
     const bool keep = store >> i & 1;
     float c[8], s[8];
-    bool have = false;
-    for (int h0 = h_begin + hb; h0 < h_end; h0 += kHeadsInFlight * head_step) {
-      uint4 xa[kHeadsInFlight], xb[kHeadsInFlight];
+    if (turns) {
+      const float4* cp = reinterpret_cast<const float4*>(turns_s + i * half + 8 * unit);
+      const float4* sp = reinterpret_cast<const float4*>(turns_s + (TOKENS + i) * half + 8 * unit);
 #pragma unroll
-      for (int k = 0; k < kHeadsInFlight; ++k) {
-        const int h = h0 + k * head_step;
-        if (h >= h_end || (h >= H && !keep)) continue;
-        const T* row = h < H ? static_cast<const T*>(p.query) + t * p.query_row_stride + (int64_t)h * d
-                     : h < H + KV ? static_cast<const T*>(p.key) + t * p.key_row_stride + (int64_t)(h - H) * d
-                                  : static_cast<const T*>(p.value) + t * p.value_row_stride + (int64_t)(h - H - KV) * d;
-        const bool value = h >= H + KV;
-        xa[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit : ca));
-        xb[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit + 8 : cb));
+      for (int j = 0; j < 2; ++j) {
+        const float4 cv = cp[j], sv = sp[j];
+        c[4 * j] = cv.x; c[4 * j + 1] = cv.y; c[4 * j + 2] = cv.z; c[4 * j + 3] = cv.w;
+        s[4 * j] = sv.x; s[4 * j + 1] = sv.y; s[4 * j + 2] = sv.z; s[4 * j + 3] = sv.w;
       }
-      if (turns && !have && h0 < H + KV) {
-        have = true;
-        const int pair = 8 * unit, axis = axis_of(p, pair);
-        if (axis_of(p, pair + 7) == axis) {
-          const int64_t pos = position_of(p, axis, t);
-          if (pos >= 0 && pos < p.rotary_positions) {
-            load_table8<T>(p, p.cos_cache, pos * half + pair, c);
-            load_table8<T>(p, p.sin_cache, pos * half + pair, s);
-          } else {
-            set_status(p.device_status, kStatusBadPosition);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              c[j] = 1.f;
-              s[j] = 0.f;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int64_t pos = position_of(p, axis_of(p, pair + j), t);
-            const bool in = pos >= 0 && pos < p.rotary_positions;
-            if (!in) set_status(p.device_status, kStatusBadPosition);
-            c[j] = in ? table_value<T>(p, p.cos_cache, pos * half + pair + j) : 1.f;
-            s[j] = in ? table_value<T>(p, p.sin_cache, pos * half + pair + j) : 0.f;
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kHeadsInFlight; ++k) {
-        const int h = h0 + k * head_step;
-        if (h >= h_end || (h >= H && !keep)) continue;
-        const bool value = h >= H + KV;
+    }
+    const T* q = static_cast<const T*>(p.query) + t * p.query_row_stride;
+    T* out = static_cast<T*>(p.output) + t * p.output_row_stride;
+#pragma unroll 2
+    for (int h = h_first; h < q_end; h += head_step) {
+      const T* row = q + h * d;
+      uint4 xa = *reinterpret_cast<const uint4*>(row + ca), xb = *reinterpret_cast<const uint4*>(row + cb);
+      if (turns) {
         float a[8], b[8];
-        unpack8<T>(xa[k], a);
-        unpack8<T>(xb[k], b);
+        unpack8<T>(xa, a);
+        unpack8<T>(xb, b);
+        turn(interleaved, c, s, a, b);
+        xa = pack8<T>(a);
+        xb = pack8<T>(b);
+      }
+      T* dst = out + h * d;
+      *reinterpret_cast<uint4*>(dst + ca) = xa;
+      *reinterpret_cast<uint4*>(dst + cb) = xb;
+    }
+    if (!keep) continue;
+    const int64_t slot = slots[i];
+    // first head of this thread past the query heads
+    for (int h = h_first + (h_first < H ? (H - h_first + head_step - 1) / head_step * head_step : 0); h < h_end; h += head_step) {
+      const bool value = h >= H + KV;
+      const int kh = value ? h - H - KV : h - H;
+      const T* row = (value ? static_cast<const T*>(p.value) + t * p.value_row_stride
+                            : static_cast<const T*>(p.key) + t * p.key_row_stride) + kh * d;
+      const int sa = value ? 16 * unit : ca, sb = value ? 16 * unit + 8 : cb;
+      uint4 xa = *reinterpret_cast<const uint4*>(row + sa), xb = *reinterpret_cast<const uint4*>(row + sb);
+      const int64_t at = (slot * KV + kh) * d;
+      void* cache = value ? p.value_cache : p.key_cache;
+      float a[8], b[8];
+      unpack8<T>(xa, a);
+      unpack8<T>(xb, b);
+      if (turns && !value) turn(interleaved, c, s, a, b);
+      if constexpr (FP8) {
+        const float scale = __ldg((value ? p.v_scale : p.k_scale) + slot / p.block_size * KV + kh);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sa) = e4m3x8(a, scale);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sb) = e4m3x8(b, scale);
+      } else {
         if (turns && !value) {
-          if (p.rotary_interleaved) {  // pairs (0,1), (2,3), .. of the 16 contiguous channels
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float y0 = a[2 * j] * c[j] - a[2 * j + 1] * s[j], y1 = a[2 * j + 1] * c[j] + a[2 * j] * s[j];
-              a[2 * j] = y0;
-              a[2 * j + 1] = y1;
-              const float z0 = b[2 * j] * c[4 + j] - b[2 * j + 1] * s[4 + j];
-              const float z1 = b[2 * j + 1] * c[4 + j] + b[2 * j] * s[4 + j];
-              b[2 * j] = z0;
-              b[2 * j + 1] = z1;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float y0 = a[j] * c[j] - b[j] * s[j], y1 = b[j] * c[j] + a[j] * s[j];
-              a[j] = y0;
-              b[j] = y1;
-            }
-          }
-          xa[k] = pack8<T>(a);
-          xb[k] = pack8<T>(b);
+          xa = pack8<T>(a);
+          xb = pack8<T>(b);
         }
-        if (h < H) {
-          T* row = static_cast<T*>(p.output) + t * p.output_row_stride + (int64_t)h * d;
-          *reinterpret_cast<uint4*>(row + ca) = xa[k];
-          *reinterpret_cast<uint4*>(row + cb) = xb[k];
-          continue;
-        }
-        const int kh = value ? h - H - KV : h - H;
-        const int64_t at = ((int64_t)sl * KV + kh) * d;
-        void* cache = value ? p.value_cache : p.key_cache;
-        const int sa = value ? 16 * unit : ca, sb = value ? 16 * unit + 8 : cb;
-        if constexpr (FP8) {
-          const float scale = __ldg((value ? p.v_scale : p.k_scale) + (int64_t)(sl / p.block_size) * KV + kh);
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sa) = e4m3x8(a, scale);
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sb) = e4m3x8(b, scale);
-        } else {
-          *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sa) = xa[k];
-          *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sb) = xb[k];
-        }
+        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sa) = xa;
+        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sb) = xb;
       }
     }
   }
@@ -413,12 +397,13 @@ void launch_vec(const B200RotaryAppendParams& p, const int* keys, const int* las
   const int cta_heads = spread ? per_pass : heads;
   const unsigned splits = (unsigned)((heads + cta_heads - 1) / cta_heads);
   const int threads = units * head_step;
+  const size_t turns = sizeof(float) * (size_t)p.rotary_dim;  // cos and sin of one token
   if (p.num_tokens < 16 * num_sms)
-    rotary_append_vec_kernel<T, FP8, 1><<<dim3(p.num_tokens, splits), threads, 0, stream>>>(p, keys, last, cap, units,
+    rotary_append_vec_kernel<T, FP8, 1><<<dim3(p.num_tokens, splits), threads, turns, stream>>>(p, keys, last, cap, units,
                                                                                            head_step, cta_heads);
   else
     rotary_append_vec_kernel<T, FP8, kScanTokens><<<dim3((p.num_tokens + kScanTokens - 1) / kScanTokens, splits), threads,
-                                                    0, stream>>>(p, keys, last, cap, units, head_step, cta_heads);
+                                                    kScanTokens * turns, stream>>>(p, keys, last, cap, units, head_step, cta_heads);
 }
 
 uint32_t table_capacity(int tokens) {
