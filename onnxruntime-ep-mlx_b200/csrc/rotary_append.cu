@@ -12,7 +12,7 @@
 // shared memory and stay in registers over the heads.  rotary_append_kernel takes what is not aligned to such units.
 //
 // Of several tokens with one slot the last is stored.  Up to B200_ROTARY_APPEND_SCAN_TOKENS tokens,
-// a CTA compares its tokens' slots with every later one (kScanTokens tokens per CTA share the reads of
+// a CTA compares its tokens' slots with every later one (up to 4 tokens per CTA share the reads of
 // the list); beyond, where that work grows with the square, a hash table is filled first.
 #include <algorithm>
 
@@ -158,38 +158,48 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(const B200RotaryAppe
 }
 
 // Whether a later token names the same slot, for the TOKENS tokens from t0 on (bit i: token t0 + i).
+// A CTA barrier.
 template <int TOKENS>
 __device__ __forceinline__ int later_same_slot(const B200RotaryAppendParams& p, int64_t t0, const int32_t (&slot)[TOKENS]) {
   const int tid = threadIdx.x, threads = blockDim.x;
   const int32_t* list = p.slot_mapping;
   const int64_t n = p.num_tokens, from = t0 + TOKENS;
-  int later = 0;
+  bool hit[TOKENS];
 #pragma unroll
-  for (int i = 0; i < TOKENS; ++i)
+  for (int i = 0; i < TOKENS; ++i) {
+    hit[i] = false;
 #pragma unroll
-    for (int j = i + 1; j < TOKENS; ++j) later |= (slot[i] == slot[j]) << i;
+    for (int j = i + 1; j < TOKENS; ++j) hit[i] |= slot[i] == slot[j];
+  }
   auto compare = [&](int32_t other) {
 #pragma unroll
-    for (int i = 0; i < TOKENS; ++i) later |= (slot[i] == other) << i;
+    for (int i = 0; i < TOKENS; ++i) hit[i] |= slot[i] == other;
   };
-  // up to the next 16-byte boundary, whole vectors, the rest
-  const int64_t head = min(n - from, (int64_t)(-(reinterpret_cast<uintptr_t>(list + from) >> 2) & 3));
-  if (tid < head) compare(__ldg(list + from + tid));
-  const int64_t vecs = from < n ? (n - from - head) / 4 : 0;
-  const int4* wide = reinterpret_cast<const int4*>(list + from + (head > 0 ? head : 0));
+  if (from < n) {  // up to the next 16-byte boundary, whole vectors, the rest
+    const int rest = (int)(n - from);
+    const int head = min(rest, (int)(-(reinterpret_cast<uintptr_t>(list + from) >> 2) & 3)), vecs = (rest - head) / 4;
+    const int32_t* first = list + from;
+    const int4* wide = reinterpret_cast<const int4*>(first + head);
+    if (tid < head) compare(__ldg(first + tid));
 #pragma unroll 4
-  for (int64_t v = tid; v < vecs; v += threads) {
-    const int4 w = __ldg(wide + v);
-    compare(w.x);
-    compare(w.y);
-    compare(w.z);
-    compare(w.w);
+    for (int v = tid; v < vecs; v += threads) {
+      const int4 w = __ldg(wide + v);
+      compare(w.x);
+      compare(w.y);
+      compare(w.z);
+      compare(w.w);
+    }
+    const int tail = head + vecs * 4 + tid;
+    if (tail < rest) compare(__ldg(first + tail));
   }
-  for (int64_t u = from + head + vecs * 4 + tid; u < n; u += threads) compare(__ldg(list + u));
-  int any = 0;
+  bool any = false;
 #pragma unroll
-  for (int i = 0; i < TOKENS; ++i) any |= (__syncthreads_or(later >> i & 1) ? 1 : 0) << i;
-  return any;
+  for (int i = 0; i < TOKENS; ++i) any |= hit[i];
+  if (!__syncthreads_or(any)) return 0;
+  int later = 0;
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) later |= (__syncthreads_or(hit[i]) ? 1 : 0) << i;
+  return later;
 }
 
 template <typename T>
@@ -224,7 +234,6 @@ __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float scale) {
 }
 
 constexpr int kVecThreads = 128;
-constexpr int kScanTokens = 4;
 
 // The cos and sin values of TOKENS tokens from t0 on into shared memory, [token][pair] each (1 and 0
 // where a position is out of range).
@@ -263,17 +272,21 @@ __device__ __forceinline__ void turn(bool interleaved, const float (&c)[8], cons
 }
 
 // CTA: TOKENS tokens x heads [blockIdx.y * cta_heads, + cta_heads) of the query, key and value heads in
-// that order; thread (unit of `units`, head offset of `head_step`).
+// that order.  A warp owns one token; a lane owns (unit of `units`, head offset), lanes past the last
+// whole head idle.  kBatch heads' loads go out before the first of them is used.
 template <typename T, bool FP8, int TOKENS>
-__global__ void __launch_bounds__(kVecThreads, 7) rotary_append_vec_kernel(const __grid_constant__ B200RotaryAppendParams p,
+__global__ void __launch_bounds__(kVecThreads, 5) rotary_append_vec_kernel(const __grid_constant__ B200RotaryAppendParams p,
                                                                             const int* keys, const int* last,
-                                                                            uint32_t capacity, int units, int head_step,
-                                                                            int cta_heads) {
+                                                                            uint32_t capacity, int units, int cta_heads) {
+  constexpr int kBatch = 4;
   const int64_t t0 = (int64_t)blockIdx.x * TOKENS;
-  const int tid = threadIdx.x, unit = tid % units, hb = tid / units;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int unit = lane % units, warp_heads = 32 / units;
   const int d = p.head_size, H = p.num_heads, KV = p.kv_num_heads, half = p.rotary_dim / 2;
-  const int h_first = blockIdx.y * cta_heads + hb, h_end = min(H + 2 * KV, (int)(blockIdx.y + 1) * cta_heads);
-  const int q_end = min(H, h_end);
+  const int i = warp % TOKENS;  // this warp's token
+  const int head_step = warp_heads * (kVecThreads / 32 / TOKENS);
+  const int h_first = blockIdx.y * cta_heads + warp / TOKENS * warp_heads + lane / units;
+  const int h_end = min(H + 2 * KV, (int)(blockIdx.y + 1) * cta_heads);
   const bool turns = unit < p.rotary_dim / 16, interleaved = p.rotary_interleaved != 0;
   // first channels of the unit's two pieces in query and key heads
   int ca, cb;
@@ -286,90 +299,115 @@ __global__ void __launch_bounds__(kVecThreads, 7) rotary_append_vec_kernel(const
     ca += ca < p.rotary_offset ? 0 : p.rotary_dim;
     cb += cb < p.rotary_offset ? 0 : p.rotary_dim;
   }
+  const int64_t t = t0 + i;
+  const bool active = t < p.num_tokens && lane / units < warp_heads;
+  const T* q = static_cast<const T*>(p.query) + t * p.query_row_stride;
+  const int q_end = active ? min(H, h_end) : 0;
+  uint4 xa[kBatch], xb[kBatch];
+  auto load_queries = [&](int h0) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int h = h0 + k * head_step;
+      if (h < q_end) {
+        xa[k] = *reinterpret_cast<const uint4*>(q + h * d + ca);
+        xb[k] = *reinterpret_cast<const uint4*>(q + h * d + cb);
+      }
+    }
+  };
+  load_queries(h_first);  // in flight during the gather and the search below
   extern __shared__ float turns_s[];  // cos [TOKENS][half], sin [TOKENS][half]
-  __shared__ int32_t slots[TOKENS];
   load_turns<T, TOKENS>(p, t0, half, turns_s, turns_s + TOKENS * half);
-  int store = 0;
+  int32_t slot = -1;
+  bool keep = false;
   if (h_end > H) {  // this CTA has rows to store
-    int32_t slot[TOKENS];
+    int32_t slots[TOKENS];
 #pragma unroll
-    for (int i = 0; i < TOKENS; ++i) {
-      slot[i] = t0 + i < p.num_tokens ? __ldg(p.slot_mapping + t0 + i) : -1;
-      const bool valid = slot[i] >= -1 && (int64_t)slot[i] < (int64_t)p.num_blocks * p.block_size;
-      if (!valid && tid == 0) set_status(p.device_status, kStatusBadSlot);
-      store |= (valid && slot[i] >= 0) << i;
-      if (tid == 0) slots[i] = slot[i];
+    for (int j = 0; j < TOKENS; ++j) {
+      slots[j] = t0 + j < p.num_tokens ? __ldg(p.slot_mapping + t0 + j) : -1;
+      if (j == i) slot = slots[j];
     }
-    if (keys) {
-#pragma unroll
-      for (int i = 0; i < TOKENS; ++i)
-        if (store >> i & 1) store &= ~((last_token(slot[i], (int)(t0 + i), keys, last, capacity) != (int)(t0 + i)) << i);
-    } else {
-      store &= ~later_same_slot<TOKENS>(p, t0, slot);
-    }
+    const bool valid = slot >= -1 && (int64_t)slot < (int64_t)p.num_blocks * p.block_size;
+    if (!valid && lane == 0) set_status(p.device_status, kStatusBadSlot);
+    keep = valid && slot >= 0;
+    if (!keys) keep &= !(later_same_slot<TOKENS>(p, t0, slots) >> i & 1);
+    else if (keep) keep = last_token(slot, (int)(t0 + i), keys, last, capacity) == (int)(t0 + i);
   }
   __syncthreads();
-#pragma unroll 1
-  for (int i = 0; i < TOKENS; ++i) {
-    const int64_t t = t0 + i;
-    if (t >= p.num_tokens) break;
-    const bool keep = store >> i & 1;
-    float c[8], s[8];
-    if (turns) {
-      const float4* cp = reinterpret_cast<const float4*>(turns_s + i * half + 8 * unit);
-      const float4* sp = reinterpret_cast<const float4*>(turns_s + (TOKENS + i) * half + 8 * unit);
+  if (!active) return;
+  float c[8], s[8];
+  if (turns) {
+    const float4* cp = reinterpret_cast<const float4*>(turns_s + i * half + 8 * unit);
+    const float4* sp = reinterpret_cast<const float4*>(turns_s + (TOKENS + i) * half + 8 * unit);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 cv = cp[j], sv = sp[j];
-        c[4 * j] = cv.x; c[4 * j + 1] = cv.y; c[4 * j + 2] = cv.z; c[4 * j + 3] = cv.w;
-        s[4 * j] = sv.x; s[4 * j + 1] = sv.y; s[4 * j + 2] = sv.z; s[4 * j + 3] = sv.w;
-      }
+    for (int j = 0; j < 2; ++j) {
+      const float4 cv = cp[j], sv = sp[j];
+      c[4 * j] = cv.x; c[4 * j + 1] = cv.y; c[4 * j + 2] = cv.z; c[4 * j + 3] = cv.w;
+      s[4 * j] = sv.x; s[4 * j + 1] = sv.y; s[4 * j + 2] = sv.z; s[4 * j + 3] = sv.w;
     }
-    const T* q = static_cast<const T*>(p.query) + t * p.query_row_stride;
-    T* out = static_cast<T*>(p.output) + t * p.output_row_stride;
-#pragma unroll 2
-    for (int h = h_first; h < q_end; h += head_step) {
-      const T* row = q + h * d;
-      uint4 xa = *reinterpret_cast<const uint4*>(row + ca), xb = *reinterpret_cast<const uint4*>(row + cb);
+  }
+  T* out = static_cast<T*>(p.output) + t * p.output_row_stride;
+  for (int h0 = h_first; h0 < q_end;) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int h = h0 + k * head_step;
+      if (h >= q_end) break;
       if (turns) {
         float a[8], b[8];
-        unpack8<T>(xa, a);
-        unpack8<T>(xb, b);
+        unpack8<T>(xa[k], a);
+        unpack8<T>(xb[k], b);
         turn(interleaved, c, s, a, b);
-        xa = pack8<T>(a);
-        xb = pack8<T>(b);
+        xa[k] = pack8<T>(a);
+        xb[k] = pack8<T>(b);
       }
-      T* dst = out + h * d;
-      *reinterpret_cast<uint4*>(dst + ca) = xa;
-      *reinterpret_cast<uint4*>(dst + cb) = xb;
+      *reinterpret_cast<uint4*>(out + h * d + ca) = xa[k];
+      *reinterpret_cast<uint4*>(out + h * d + cb) = xb[k];
     }
-    if (!keep) continue;
-    const int64_t slot = slots[i];
-    // first head of this thread past the query heads
-    for (int h = h_first + (h_first < H ? (H - h_first + head_step - 1) / head_step * head_step : 0); h < h_end; h += head_step) {
-      const bool value = h >= H + KV;
-      const int kh = value ? h - H - KV : h - H;
-      const T* row = (value ? static_cast<const T*>(p.value) + t * p.value_row_stride
-                            : static_cast<const T*>(p.key) + t * p.key_row_stride) + kh * d;
+    h0 += kBatch * head_step;
+    load_queries(h0);
+  }
+  if (!keep) return;
+  // this lane's first key or value head
+  int h0 = h_first + (h_first < H ? (H - h_first + head_step - 1) / head_step * head_step : 0);
+  const T* krow = static_cast<const T*>(p.key) + t * p.key_row_stride;
+  const T* vrow = static_cast<const T*>(p.value) + t * p.value_row_stride;
+  const int64_t at = (int64_t)slot * KV * d;  // cache row of the token
+  for (; h0 < h_end; h0 += kBatch * head_step) {
+    float scale[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int kh = h0 + k * head_step - H;
+      if (kh + H >= h_end) break;
+      const bool value = kh >= KV;
+      const T* row = value ? vrow + (kh - KV) * d : krow + kh * d;
+      xa[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit : ca));
+      xb[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit + 8 : cb));
+      if constexpr (FP8)
+        scale[k] = __ldg((value ? p.v_scale - KV : p.k_scale) + (int64_t)(slot / p.block_size) * KV + kh);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int kh = h0 + k * head_step - H;
+      if (kh + H >= h_end) break;
+      const bool value = kh >= KV;
+      const int64_t row = at + (value ? kh - KV : kh) * d;
       const int sa = value ? 16 * unit : ca, sb = value ? 16 * unit + 8 : cb;
-      uint4 xa = *reinterpret_cast<const uint4*>(row + sa), xb = *reinterpret_cast<const uint4*>(row + sb);
-      const int64_t at = (slot * KV + kh) * d;
       void* cache = value ? p.value_cache : p.key_cache;
       float a[8], b[8];
-      unpack8<T>(xa, a);
-      unpack8<T>(xb, b);
+      if (FP8 || (turns && !value)) {
+        unpack8<T>(xa[k], a);
+        unpack8<T>(xb[k], b);
+      }
       if (turns && !value) turn(interleaved, c, s, a, b);
       if constexpr (FP8) {
-        const float scale = __ldg((value ? p.v_scale : p.k_scale) + slot / p.block_size * KV + kh);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sa) = e4m3x8(a, scale);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at + sb) = e4m3x8(b, scale);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + row + sa) = e4m3x8(a, scale[k]);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + row + sb) = e4m3x8(b, scale[k]);
       } else {
         if (turns && !value) {
-          xa = pack8<T>(a);
-          xb = pack8<T>(b);
+          xa[k] = pack8<T>(a);
+          xb[k] = pack8<T>(b);
         }
-        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sa) = xa;
-        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at + sb) = xb;
+        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + row + sa) = xa[k];
+        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + row + sb) = xb[k];
       }
     }
   }
@@ -382,28 +420,30 @@ bool vector_form(const B200RotaryAppendParams& p) {
                           reinterpret_cast<uintptr_t>(p.key_cache) | reinterpret_cast<uintptr_t>(p.value_cache) |
                           reinterpret_cast<uintptr_t>(p.cos_cache) | reinterpret_cast<uintptr_t>(p.sin_cache);
   const int64_t strides = p.query_row_stride | p.key_row_stride | p.value_row_stride | p.output_row_stride;
-  return bases % 16 == 0 && strides % 8 == 0 && p.head_size % 16 == 0 && p.head_size / 16 <= kVecThreads &&
+  return bases % 16 == 0 && strides % 8 == 0 && p.head_size % 16 == 0 && p.head_size / 16 <= 32 &&
          p.rotary_dim % 16 == 0 && p.rotary_offset % 8 == 0;
 }
 
 template <typename T, bool FP8>
 void launch_vec(const B200RotaryAppendParams& p, const int* keys, const int* last, uint32_t cap, int num_sms,
                 cudaStream_t stream) {
-  const int units = p.head_size / 16, head_step = kVecThreads / units, heads = p.num_heads + 2 * p.kv_num_heads;
-  const int per_pass = head_step;
-  // Few tokens: heads spread over CTAs, one per thread, for the shortest chain of loads.
-  const int64_t one_pass = (int64_t)p.num_tokens * ((heads + per_pass - 1) / per_pass);
-  const bool spread = one_pass <= 8 * (int64_t)num_sms;
-  const int cta_heads = spread ? per_pass : heads;
-  const unsigned splits = (unsigned)((heads + cta_heads - 1) / cta_heads);
-  const int threads = units * head_step;
+  const int units = p.head_size / 16, heads = p.num_heads + 2 * p.kv_num_heads;
   const size_t turns = sizeof(float) * (size_t)p.rotary_dim;  // cos and sin of one token
-  if (p.num_tokens < 16 * num_sms)
-    rotary_append_vec_kernel<T, FP8, 1><<<dim3(p.num_tokens, splits), threads, turns, stream>>>(p, keys, last, cap, units,
-                                                                                           head_step, cta_heads);
-  else
-    rotary_append_vec_kernel<T, FP8, kScanTokens><<<dim3((p.num_tokens + kScanTokens - 1) / kScanTokens, splits), threads,
-                                                    kScanTokens * turns, stream>>>(p, keys, last, cap, units, head_step, cta_heads);
+  if (p.num_tokens < 16 * num_sms) {
+    // Few tokens: a token's heads spread over CTAs, one per lane, while that leaves the SMs at most 8
+    // CTAs each, for the shortest chain of loads.
+    const int pass = 32 / units * (kVecThreads / 32);
+    const unsigned passes = (unsigned)((heads + pass - 1) / pass);
+    const bool spread = (int64_t)p.num_tokens * passes <= 8 * (int64_t)num_sms;
+    rotary_append_vec_kernel<T, FP8, 1><<<dim3(p.num_tokens, spread ? passes : 1), kVecThreads, turns, stream>>>(
+        p, keys, last, cap, units, spread ? pass : heads);
+  } else if (p.num_tokens < 48 * num_sms) {  // smaller CTAs fill the last wave better
+    rotary_append_vec_kernel<T, FP8, 2><<<dim3((p.num_tokens + 1) / 2), kVecThreads, 2 * turns, stream>>>(
+        p, keys, last, cap, units, heads);
+  } else {  // 4 tokens share the reads of the slot list
+    rotary_append_vec_kernel<T, FP8, 4><<<dim3((p.num_tokens + 3) / 4), kVecThreads, 4 * turns, stream>>>(
+        p, keys, last, cap, units, heads);
+  }
 }
 
 uint32_t table_capacity(int tokens) {
