@@ -11,7 +11,6 @@ first on a stream, allocate their status word and scratch: make them before a gr
 from __future__ import annotations
 
 import ctypes
-import functools
 import struct
 
 import torch
@@ -24,6 +23,7 @@ _FP8 = torch.float8_e4m3fn
 _ACT = {torch.float16: _capi.DTYPE_FLOAT16, torch.bfloat16: _capi.DTYPE_BFLOAT16}
 _TABLE = {**_ACT, torch.float32: _capi.DTYPE_FLOAT}
 _INDEX = {torch.int32: _capi.DTYPE_INT32, torch.int64: _capi.DTYPE_INT64}
+_DENSE = torch.contiguous_format
 _E4M3 = _capi.DTYPE_FLOAT8E4M3FN
 
 # The parameter structs of include/b200_layer.h as packed bytes (a decode step makes these calls for
@@ -62,18 +62,10 @@ def _status_ptr(device: int) -> int:
     return pointer
 
 
-def _on_stream(fn):
-    """Give ``fn`` a ``stream`` argument: it runs with that stream current, so what it allocates belongs
-    to the stream that uses it."""
-
-    @functools.wraps(fn)
-    def wrapped(*args, stream=None, **kwargs):
-        if stream is None:
-            return fn(*args, **kwargs)
-        with torch.cuda.stream(stream):
-            return fn(*args, **kwargs)
-
-    return wrapped
+def _on_stream(stream, fn, *args, **kwargs):
+    """``fn`` with ``stream`` current, so what it allocates belongs to the stream that uses it."""
+    with torch.cuda.stream(stream):
+        return fn(*args, **kwargs)
 
 
 def _call(entry, params, device, check_status=False):
@@ -114,39 +106,36 @@ def _call_with_scratch(op, entry, size_entry, layout, fields, device, workspace,
             kept.append(torch.empty(size, dtype=torch.uint8, device=f"cuda:{device}"))
 
 
-def _same_device(op, device, names, tensors):
-    """Every tensor (or None) is on CUDA device ``device``."""
+def _rows(op, name, t, rows, width, dtype, device):
+    """Row stride of a [rows, width] tensor of ``dtype`` on ``device`` whose rows are contiguous."""
+    if t.dtype is dtype and t.get_device() == device and t.shape == (rows, width):
+        if t.is_contiguous():
+            return width
+        stride, inner = t.stride()
+        if (inner == 1 or width == 1) and (stride != 0 or rows == 1):
+            return stride if rows > 1 else width
+        if stride == 0:  # the library reads a stride of 0 as dense rows
+            raise _bad(f"{op}: {name} must not be a broadcast row")
+        raise _bad(f"{op}: {name} rows must be contiguous")
+    raise _bad(f"{op}: {name} must be a [{rows}, {width}] tensor of {dtype} on cuda:{device}")
+
+
+def _dense(op, name, t, shape, dtype, device):
+    """Address of a contiguous tensor of this shape and type on ``device``."""
+    if t is not None and t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.shape == shape:
+        return t.data_ptr()
+    raise _bad(f"{op}: {name} must be a contiguous {tuple(shape)} tensor of {dtype} on cuda:{device}")
+
+
+def _device(op, t):
+    device = t.get_device()
     if device < 0:
         raise _bad(f"{op}: tensors must be on a CUDA device")
-    for i, t in enumerate(tensors):
-        if t is not None and t.get_device() != device:
-            raise _bad(f"{op}: {names.split()[i]} is on another device")
+    return device
 
 
-def _rows(op, name, t, rows, width, dtype):
-    """Row stride of a [rows, width] tensor of ``dtype`` whose rows are contiguous."""
-    if t.dtype != dtype or t.shape != (rows, width):
-        raise _bad(f"{op}: {name} must be a [{rows}, {width}] tensor of {dtype}")
-    if rows <= 1:
-        if width > 1 and t.stride(1) != 1:
-            raise _bad(f"{op}: {name} rows must be contiguous")
-        return width
-    stride, inner = t.stride()
-    if inner != 1 and width > 1:
-        raise _bad(f"{op}: {name} rows must be contiguous")
-    if stride == 0:  # the library reads a stride of 0 as dense rows
-        raise _bad(f"{op}: {name} must not be a broadcast row")
-    return stride
-
-
-def _dense(op, name, t, shape, dtype):
-    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
-        raise _bad(f"{op}: {name} must be a contiguous {tuple(shape)} tensor of {dtype}")
-
-
-@_on_stream
 def skip_rms_norm(x, residual, weight, *, epsilon=1e-6, out_dtype=None, group_size=0, output=None, scales=None,
-                  residual_output=None):
+                  residual_output=None, stream=None):
     """``s = x + residual`` (fp32), ``y = s / sqrt(mean(s^2) + epsilon) * weight`` per row.
 
     ``x`` and ``residual`` (or ``None``) are ``[rows, hidden]`` in fp16 / bf16 with contiguous rows.
@@ -154,55 +143,51 @@ def skip_rms_norm(x, residual, weight, *, epsilon=1e-6, out_dtype=None, group_si
     ``(codes, scales, s in x's type)``: ``codes * scales`` stands for ``y``, ``scales`` is fp32
     ``[rows, groups]`` with one scale per row (``group_size=0``) or per ``group_size`` channels.
     """
+    if stream is not None:
+        return _on_stream(stream, skip_rms_norm, x, residual, weight, epsilon=epsilon, out_dtype=out_dtype,
+                          group_size=group_size, output=output, scales=scales, residual_output=residual_output)
     op = "SkipRmsNorm"
     dtype = x.dtype
     act = _ACT.get(dtype)
     if act is None or x.dim() != 2:
         raise _bad(f"{op}: x must be a [rows, hidden] tensor of fp16 or bf16")
     rows, hidden = x.shape
-    device = x.get_device()
-    _same_device(op, device, "residual weight output scales residual_output",
-                 (residual, weight, output, scales, residual_output))
-    stride = _rows(op, "x", x, rows, hidden, dtype)
+    device = _device(op, x)
+    stride = _rows(op, "x", x, rows, hidden, dtype, device)
     r_ptr = r_stride = s_ptr = 0
     if residual is not None:
-        r_stride = _rows(op, "residual", residual, rows, hidden, dtype)
+        r_stride = _rows(op, "residual", residual, rows, hidden, dtype, device)
         r_ptr = residual.data_ptr()
-    _dense(op, "weight", weight, (hidden,), dtype)
-    if out_dtype is None or out_dtype == dtype:
-        fp8, out_dtype = False, dtype
-    elif out_dtype == _FP8:
-        fp8 = True
-    else:
+    w_ptr = _dense(op, "weight", weight, (hidden,), dtype, device)
+    fp8 = out_dtype is _FP8
+    if not fp8 and out_dtype is not None and out_dtype is not dtype:
         raise _bad(f"{op}: out_dtype must be x's type or float8_e4m3fn")
+    o_stride = ro_stride = hidden
     if output is None:
-        output = x.new_empty((rows, hidden), dtype=out_dtype)
-        o_stride = hidden
+        output = torch.empty_like(x, dtype=_FP8, memory_format=_DENSE) if fp8 else torch.empty_like(x, memory_format=_DENSE)
     else:
-        o_stride = _rows(op, "output", output, rows, hidden, out_dtype)
+        o_stride = _rows(op, "output", output, rows, hidden, _FP8 if fp8 else dtype, device)
     if fp8:
         groups = -(-hidden // group_size) if group_size > 0 else 1
         if scales is None:
             scales = x.new_empty((rows, groups), dtype=torch.float32)
+            s_ptr = scales.data_ptr()
         else:
-            _dense(op, "scales", scales, (rows, groups), torch.float32)
-        s_ptr = scales.data_ptr()
+            s_ptr = _dense(op, "scales", scales, (rows, groups), torch.float32, device)
     if residual_output is None:
-        residual_output = x.new_empty((rows, hidden))
-        ro_stride = hidden
+        residual_output = torch.empty_like(x, memory_format=_DENSE)
     else:
-        ro_stride = _rows(op, "residual_output", residual_output, rows, hidden, dtype)
+        ro_stride = _rows(op, "residual_output", residual_output, rows, hidden, dtype, device)
     params = _NORM.pack(rows, hidden, act, _E4M3 if fp8 else act, group_size, epsilon, stride, r_stride, o_stride,
-                        ro_stride, x.data_ptr(), r_ptr, weight.data_ptr(), output.data_ptr(), s_ptr,
+                        ro_stride, x.data_ptr(), r_ptr, w_ptr, output.data_ptr(), s_ptr,
                         residual_output.data_ptr())
     _call(LIB.b200_skip_rms_norm, params, device)
     return (output, scales, residual_output) if fp8 else (output, residual_output)
 
 
-@_on_stream
 def rotary_append(query, key, value, key_cache, value_cache, position_ids, cos_cache, sin_cache, slot_mapping, *,
                   num_heads, kv_num_heads, axis_sections=None, rotary_interleaved=0, rotary_offset=0, k_scale=None,
-                  v_scale=None, output=None, workspace=None, check_status=False):
+                  v_scale=None, output=None, workspace=None, check_status=False, stream=None):
     """Rotate the new queries and keys and append keys and values to the paged caches (in place).
 
     ``query`` is ``[tokens, num_heads * d]``; ``key`` and ``value`` are ``[tokens, kv_num_heads * d]``,
@@ -213,6 +198,11 @@ def rotary_append(query, key, value, key_cache, value_cache, position_ids, cos_c
     of several tokens with one slot the last is stored.  fp8 e4m3 caches take ``k_scale`` and
     ``v_scale`` ``[blocks, kv_num_heads]``.  Returns ``(rotated query, key_cache, value_cache)``.
     """
+    if stream is not None:
+        return _on_stream(stream, rotary_append, query, key, value, key_cache, value_cache, position_ids, cos_cache,
+                          sin_cache, slot_mapping, num_heads=num_heads, kv_num_heads=kv_num_heads,
+                          axis_sections=axis_sections, rotary_interleaved=rotary_interleaved, rotary_offset=rotary_offset,
+                          k_scale=k_scale, v_scale=v_scale, output=output, workspace=workspace, check_status=check_status)
     op = "RotaryAppend"
     dtype = query.dtype
     act = _ACT.get(dtype)
@@ -224,65 +214,61 @@ def rotary_append(query, key, value, key_cache, value_cache, position_ids, cos_c
         raise _bad(f"{op}: key_cache must be [blocks, block_size, kv_num_heads, head_size]")
     nt = query.shape[0]
     blocks, block_size, _, d = shape
-    device = query.get_device()
-    _same_device(op, device, "key value key_cache value_cache position_ids cos_cache sin_cache slot_mapping k_scale "
-                 "v_scale output", (key, value, key_cache, value_cache, position_ids, cos_cache, sin_cache,
-                                    slot_mapping, k_scale, v_scale, output))
+    device = _device(op, query)
     q_ptr = query.data_ptr()
     if key is None and value is None:
-        q_stride = k_stride = v_stride = _rows(op, "packed query", query, nt, (H + 2 * KV) * d, dtype)
+        q_stride = k_stride = v_stride = _rows(op, "packed query", query, nt, (H + 2 * KV) * d, dtype, device)
         k_ptr, v_ptr = q_ptr + 2 * H * d, q_ptr + 2 * (H + KV) * d
     elif key is None or value is None:
         raise _bad(f"{op}: key and value must be given together")
     else:
-        q_stride = _rows(op, "query", query, nt, H * d, dtype)
-        k_stride = _rows(op, "key", key, nt, KV * d, dtype)
-        v_stride = _rows(op, "value", value, nt, KV * d, dtype)
+        q_stride = _rows(op, "query", query, nt, H * d, dtype, device)
+        k_stride = _rows(op, "key", key, nt, KV * d, dtype, device)
+        v_stride = _rows(op, "value", value, nt, KV * d, dtype, device)
         k_ptr, v_ptr = key.data_ptr(), value.data_ptr()
+    kc_ptr = _dense(op, "key_cache", key_cache, shape, key_cache.dtype, device)
+    vc_ptr = _dense(op, "value_cache", value_cache, shape, key_cache.dtype, device)
     cache = _DTYPES.get(key_cache.dtype)
-    if value_cache.dtype != key_cache.dtype or value_cache.shape != shape or not (
-            key_cache.is_contiguous() and value_cache.is_contiguous()):
-        raise _bad(f"{op}: key_cache and value_cache must be contiguous and alike")
     ks_ptr = vs_ptr = 0
     if cache != act:
         if cache != _E4M3:
             raise _bad(f"{op}: the cache must have the activations' type or fp8 e4m3")
-        if k_scale is None or v_scale is None:
-            raise _bad(f"{op}: fp8 caches require k_scale and v_scale")
-        _dense(op, "k_scale", k_scale, (blocks, KV), torch.float32)
-        _dense(op, "v_scale", v_scale, (blocks, KV), torch.float32)
-        ks_ptr, vs_ptr = k_scale.data_ptr(), v_scale.data_ptr()
+        ks_ptr = _dense(op, "k_scale", k_scale, (blocks, KV), torch.float32, device)
+        vs_ptr = _dense(op, "v_scale", v_scale, (blocks, KV), torch.float32, device)
     table = _TABLE.get(cos_cache.dtype)
-    if (table is None or cos_cache.dim() != 2 or sin_cache.dtype != cos_cache.dtype
-            or sin_cache.shape != cos_cache.shape or not (cos_cache.is_contiguous() and sin_cache.is_contiguous())):
-        raise _bad(f"{op}: cos_cache and sin_cache must be contiguous [positions, rotary_dim / 2] tensors alike")
-    positions, half = cos_cache.shape
+    tables = cos_cache.shape
+    if table is None or len(tables) != 2:
+        raise _bad(f"{op}: cos_cache must be [positions, rotary_dim / 2] of the activations' type or fp32")
+    positions, half = tables
+    cos_ptr = _dense(op, "cos_cache", cos_cache, tables, cos_cache.dtype, device)
+    sin_ptr = _dense(op, "sin_cache", sin_cache, tables, cos_cache.dtype, device)
     index = _INDEX.get(position_ids.dtype)
-    rank = position_ids.dim()
-    if index is None or rank not in (1, 2) or position_ids.shape[-1] != nt:
-        raise _bad(f"{op}: position_ids must be an int32 or int64 [tokens] or [axes, tokens] tensor")
-    if nt > 1 and position_ids.stride(-1) == 0:  # the library reads a token stride of 0 as 1
-        position_ids = position_ids.contiguous()
-    axes = 1 if rank == 1 else position_ids.shape[0]
-    if axis_sections is None:
-        sections = (half, 0, 0, 0)
-        named = 1
+    places = position_ids.shape
+    rank = len(places)
+    if index is None or rank not in (1, 2) or places[-1] != nt or position_ids.get_device() != device:
+        raise _bad(f"{op}: position_ids must be an int32 or int64 [tokens] or [axes, tokens] tensor on cuda:{device}")
+    if position_ids.is_contiguous():
+        axis_stride, token_stride = nt, 1
     else:
-        named = len(axis_sections)
-        sections = (*axis_sections, 0, 0, 0)[:4]
+        if nt > 1 and position_ids.stride(-1) == 0:  # the library reads a token stride of 0 as 1
+            position_ids = position_ids.contiguous()
+        axis_stride, token_stride = position_ids.stride(0), position_ids.stride(-1)
+    axes = 1 if rank == 1 else places[0]
+    if axis_sections is None:
+        named, sections = 1, (half, 0, 0, 0)
+    else:
+        named, sections = len(axis_sections), (*axis_sections, 0, 0, 0)[:4]
     if named != axes or axes > 4:
         raise _bad(f"{op}: axis_sections must name the pairs of each of the {axes} position axes (at most 4)")
-    _dense(op, "slot_mapping", slot_mapping, (nt,), torch.int32)
+    slot_ptr = _dense(op, "slot_mapping", slot_mapping, (nt,), torch.int32, device)
     if output is None:
-        output = query.new_empty((nt, H * d))
+        output = torch.empty_like(query, memory_format=_DENSE) if key is not None else query.new_empty((nt, H * d))
         o_stride = H * d
     else:
-        o_stride = _rows(op, "output", output, nt, H * d, dtype)
+        o_stride = _rows(op, "output", output, nt, H * d, dtype, device)
     fields = (H, KV, d, 2 * half, rotary_offset, rotary_interleaved, positions, axes, *sections, act, cache, table, index,
-              nt, blocks, block_size, q_stride, k_stride, v_stride, o_stride, position_ids.stride(0) if rank == 2 else 0,
-              position_ids.stride(-1), q_ptr, k_ptr, v_ptr, output.data_ptr(), key_cache.data_ptr(),
-              value_cache.data_ptr(), position_ids.data_ptr(), cos_cache.data_ptr(), sin_cache.data_ptr(),
-              slot_mapping.data_ptr(), ks_ptr, vs_ptr)
+              nt, blocks, block_size, q_stride, k_stride, v_stride, o_stride, axis_stride, token_stride, q_ptr, k_ptr, v_ptr,
+              output.data_ptr(), kc_ptr, vc_ptr, position_ids.data_ptr(), cos_ptr, sin_ptr, slot_ptr, ks_ptr, vs_ptr)
     if nt <= _capi.ROTARY_APPEND_SCAN_TOKENS:
         _call(LIB.b200_rotary_append, _ROPE.pack(*fields, 0, 0, _status_ptr(device)), device, check_status)
     else:
@@ -291,10 +277,9 @@ def rotary_append(query, key, value, key_cache, value_cache, position_ids, cos_c
     return output, key_cache, value_cache
 
 
-@_on_stream
 def shared_prefix_attention(query, key_cache, value_cache, cumulative_sequence_length, past_seqlens, block_table,
                             prefix_block_table, *, prefix_length, num_heads, kv_num_heads, scale=0.0, softcap=0.0,
-                            head_sink=None, output=None, workspace=None, num_sms=0, check_status=False):
+                            head_sink=None, output=None, workspace=None, num_sms=0, check_status=False, stream=None):
     """Causal attention of a batch whose sequences share the ``prefix_length`` keys of
     ``prefix_block_table``; sequence ``b`` continues with its own ``past_seqlens[b]`` keys and its new
     tokens, paged by row ``b`` of ``block_table``.
@@ -304,6 +289,11 @@ def shared_prefix_attention(query, key_cache, value_cache, cumulative_sequence_l
     ``[tokens, num_heads * d]``.  The scratch is the current stream's own buffer unless ``workspace``
     (uint8, at least ``b200_shared_prefix_attention_workspace_size`` bytes) is given.
     """
+    if stream is not None:
+        return _on_stream(stream, shared_prefix_attention, query, key_cache, value_cache, cumulative_sequence_length,
+                          past_seqlens, block_table, prefix_block_table, prefix_length=prefix_length, num_heads=num_heads,
+                          kv_num_heads=kv_num_heads, scale=scale, softcap=softcap, head_sink=head_sink, output=output,
+                          workspace=workspace, num_sms=num_sms, check_status=check_status)
     op = "SharedPrefixAttention"
     dtype = query.dtype
     act = _ACT.get(dtype)
@@ -315,37 +305,29 @@ def shared_prefix_attention(query, key_cache, value_cache, cumulative_sequence_l
         raise _bad(f"{op}: key_cache must be [blocks, block_size, kv_num_heads, head_size]")
     nt = query.shape[0]
     blocks, block_size, _, d = shape
-    device = query.get_device()
-    _same_device(op, device, "key_cache value_cache cumulative_sequence_length past_seqlens block_table "
-                 "prefix_block_table head_sink output", (key_cache, value_cache, cumulative_sequence_length, past_seqlens,
-                                                         block_table, prefix_block_table, head_sink, output))
-    if value_cache.shape != shape or key_cache.dtype != dtype or value_cache.dtype != dtype or not (
-            key_cache.is_contiguous() and value_cache.is_contiguous()):
-        raise _bad(f"{op}: key_cache and value_cache must be contiguous, alike and of the query's type")
-    batch = past_seqlens.shape[0] if past_seqlens.dim() == 1 else -1
-    if block_table.dim() != 2 or block_table.shape[0] != batch:
-        raise _bad(f"{op}: inconsistent cumulative lengths, past lengths or block table")
-    columns = block_table.shape[1]
-    _dense(op, "past_seqlens", past_seqlens, (batch,), torch.int32)
-    _dense(op, "cumulative_sequence_length", cumulative_sequence_length, (batch + 1,), torch.int32)
-    _dense(op, "block_table", block_table, (batch, columns), torch.int32)
+    device = _device(op, query)
+    q_stride = _rows(op, "query", query, nt, H * d, dtype, device)
+    kc_ptr = _dense(op, "key_cache", key_cache, shape, dtype, device)
+    vc_ptr = _dense(op, "value_cache", value_cache, shape, dtype, device)
+    if block_table.dim() != 2:
+        raise _bad(f"{op}: block_table must be [batch, blocks]")
+    batch, columns = tables = block_table.shape
+    bt_ptr = _dense(op, "block_table", block_table, tables, torch.int32, device)
+    past_ptr = _dense(op, "past_seqlens", past_seqlens, (batch,), torch.int32, device)
+    cum_ptr = _dense(op, "cumulative_sequence_length", cumulative_sequence_length, (batch + 1,), torch.int32, device)
     pt_ptr = prefix_blocks = sink_ptr = 0
     if prefix_block_table is not None:
         prefix_blocks = prefix_block_table.numel()
-        _dense(op, "prefix_block_table", prefix_block_table, (prefix_blocks,), torch.int32)
-        pt_ptr = prefix_block_table.data_ptr()
+        pt_ptr = _dense(op, "prefix_block_table", prefix_block_table, (prefix_blocks,), torch.int32, device)
     if head_sink is not None:
-        _dense(op, "head_sink", head_sink, (H,), dtype)
-        sink_ptr = head_sink.data_ptr()
-    q_stride = _rows(op, "query", query, nt, H * d, dtype)
+        sink_ptr = _dense(op, "head_sink", head_sink, (H,), dtype, device)
     if output is None:
-        output = query.new_empty((nt, H * d))
+        output = torch.empty_like(query, memory_format=_DENSE)
         o_stride = H * d
     else:
-        o_stride = _rows(op, "output", output, nt, H * d, dtype)
+        o_stride = _rows(op, "output", output, nt, H * d, dtype, device)
     fields = (H, KV, d, scale, softcap, act, nt, batch, blocks, block_size, columns, prefix_length, prefix_blocks, num_sms,
-              q_stride, o_stride, query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-              cumulative_sequence_length.data_ptr(), past_seqlens.data_ptr(), block_table.data_ptr(), pt_ptr, sink_ptr,
+              q_stride, o_stride, query.data_ptr(), kc_ptr, vc_ptr, cum_ptr, past_ptr, bt_ptr, pt_ptr, sink_ptr,
               output.data_ptr())
     _call_with_scratch(op, LIB.b200_shared_prefix_attention, LIB.b200_shared_prefix_attention_workspace_size, _PREFIX,
                        fields, device, workspace, check_status)
