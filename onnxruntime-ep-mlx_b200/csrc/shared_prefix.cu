@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
   const B200SharedPrefixParams& p = a.p;
   release_dependents();
   const int tid = threadIdx.x, lane = tid & 31;
-  for (int t = tid; t < p.num_tokens; t += kPlanThreads) a.token_seq[t] = -1;
+  for (int t = tid; t < p.num_tokens; t += kPlanThreads) a.token_info[t] = make_int4(0, -1, 0, 0);
   if (tid == 0) *a.next_item = 0;
   __syncthreads();
   int2 carry = make_int2(0, 0);
@@ -187,19 +187,21 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
       if ((int64_t)nq * a.group <= a.own_rows) work.x = nq ? (int)((total + kOwnTile - 1) / kOwnTile) : 0;
       else work.y = (nq + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
     }
-    if (nq <= 32)
-      for (int i = 0; i < nq; ++i) a.token_seq[c0 + i] = b;
-    for (unsigned left = __ballot_sync(0xffffffffu, nq > 32); left; left &= left - 1) {  // long ones: the whole warp
-      const int src = __ffs(left) - 1;
-      const int first = __shfl_sync(0xffffffffu, c0, src), n = __shfl_sync(0xffffffffu, nq, src);
-      const int seq = __shfl_sync(0xffffffffu, b, src);
-      for (int i = lane; i < n; i += 32) a.token_seq[first + i] = seq;
-    }
     int2 total;
     const int2 incl = block_inclusive_sum(work, warp_sums, total);
+    const int first = carry.x + incl.x - work.x;
     if (b < p.batch) {
-      a.seq_tiles[b] = carry.x + incl.x - work.x;
+      a.seq_tiles[b] = first;
       a.seq_pairs[b] = carry.y + incl.y - work.y;
+    }
+    const int4 info = make_int4(c0, nq, first, work.x);
+    if (nq <= 32)
+      for (int i = 0; i < nq; ++i) a.token_info[c0 + i] = info;
+    for (unsigned left = __ballot_sync(0xffffffffu, nq > 32); left; left &= left - 1) {  // long ones: the whole warp
+      const int src = __ffs(left) - 1;
+      const int4 seq = make_int4(__shfl_sync(0xffffffffu, info.x, src), __shfl_sync(0xffffffffu, info.y, src),
+                                 __shfl_sync(0xffffffffu, info.z, src), __shfl_sync(0xffffffffu, info.w, src));
+      for (int i = lane; i < seq.y; i += 32) a.token_info[seq.x + i] = seq;
     }
     carry.x += total.x;
     carry.y += total.y;
@@ -211,108 +213,95 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Merge: one warp per (token, head) row joins the row's triples.
+// Merge: D / 4 lanes per (token, head) row join the row's triples, kMergeBatch of them in flight.
+// Bound by the slabs' reads, which come from L2 as far as the own keys' stream has left them there.
 // ---------------------------------------------------------------------------------------------
-constexpr int kMergeWarps = 8;
+constexpr int kMergeThreads = 128;
+constexpr int kMergeBatch = 8;
 constexpr float kLog2eMerge = 1.4426950408889634f;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kMergeWarps) shared_prefix_merge_kernel(const SharedPrefixArgs a, int vector_rows) {
-  constexpr int C = D / 32;  // channels per lane
+__global__ void __launch_bounds__(kMergeThreads) shared_prefix_merge_kernel(const SharedPrefixArgs a, int vector_rows) {
+  constexpr int kLanes = D / 4;
   const B200SharedPrefixParams& p = a.p;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  const int c = threadIdx.x % kLanes * 4;  // first of this lane's channels
+  const int64_t row = (int64_t)blockIdx.x * (kMergeThreads / kLanes) + threadIdx.x / kLanes;
   wait_previous();
   if (row >= a.rows) return;
   const int64_t t = row / p.num_heads;
-  const int h = (int)(row % p.num_heads), kh = h / a.group;
-  // own part: the slab, or `pieces` warps' rows
-  const int b = a.token_seq[t];
-  int own = 0;  // triples of the own keys
+  const int h = (int)(row - t * p.num_heads);
+  // own part: the slab, or `pieces` rows of the own kernel's warps
+  const int4 info = __ldcg(a.token_info + t);
+  int own = info.y > 0;
   bool cut = false;
-  int64_t w_first = 0, first_row = 0, next_row = 0;
-  if (b >= 0) {
-    own = 1;
-    const int c0 = p.cumulative_sequence_length[b], nq = p.cumulative_sequence_length[b + 1] - c0;
-    if ((int64_t)nq * a.group <= a.own_rows) {
-      const int KV = p.kv_num_heads;
-      const int64_t first = a.seq_tiles[b], tiles = a.seq_tiles[b + 1] - first;
-      const int64_t T_all = (int64_t)a.seq_tiles[p.batch] * KV, W = own_active_warps(T_all, a.own_warps);
-      const int64_t start = first * KV + kh * tiles;
-      w_first = own_warp_of(start, T_all, W);
-      own = (int)(own_warp_of(start + tiles - 1, T_all, W) - w_first + 1);
-      cut = own > 1;
-      // a warp's row block 0 holds the piece its range starts with, block 1 its last one
-      const int64_t r = (t - c0) * a.group + h % a.group;
-      first_row = (w_first * 2 + (start > own_range_start(w_first, T_all, W) ? 1 : 0)) * a.own_rows + r;
-      next_row = (w_first + 1) * 2 * a.own_rows + r;
-    }
+  int64_t first_row = 0, next_row = 0;
+  if (info.w > 0) {
+    const int KV = p.kv_num_heads, kh = h / a.group;
+    const OwnRanges ranges((int64_t)__ldcg(a.seq_tiles + p.batch) * KV, a.own_warps);
+    const int64_t start = (int64_t)info.z * KV + (int64_t)kh * info.w;
+    const int64_t w_first = ranges.warp_of(start);
+    own = (int)(ranges.warp_of(start + info.w - 1) - w_first + 1);
+    cut = own > 1;
+    // a warp's row block 0 holds the piece its range starts with, block 1 its last one
+    const int64_t r = (t - info.x) * a.group + h - kh * a.group;
+    first_row = (w_first * 2 + (start > ranges.start(w_first) ? 1 : 0)) * a.own_rows + r;
+    next_row = (w_first + 1) * 2 * a.own_rows + r;
   }
   const int parts = a.splits + own;
-  auto locate = [&](int i) -> int64_t {  // row of triple i in its array; cut pieces are i >= splits
-    if (!cut || i < a.splits) return (int64_t)i * a.rows + row;
-    const int piece = i - a.splits;
-    return piece == 0 ? first_row : next_row + (int64_t)(piece - 1) * 2 * a.own_rows;
-  };
-  auto triple = [&](int i) -> float2 {
-    return __ldcg((cut && i >= a.splits ? a.warp_ml : a.slab_ml) + locate(i));
-  };
-  const float sink = p.head_sink ? act<T>::to_f(static_cast<const T*>(p.head_sink)[h]) * kLog2eMerge : -INFINITY;
-  float top = sink;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, triple(i).x);
+  float top = -INFINITY, sum = 0.f;
+  if (p.head_sink) {
+    top = act<T>::to_f(static_cast<const T*>(p.head_sink)[h]) * kLog2eMerge;
+    sum = 1.f;
+  }
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = 0; base < parts; base += kMergeBatch) {
+    float2 ml[kMergeBatch];
+    float4 o[kMergeBatch];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (top == -INFINITY) top = 0.f;
-  float sum = 0.f, acc[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) acc[c] = 0.f;
-  for (int base = 0; base < parts; base += 32) {
-    float weight = 0.f;
-    if (base + lane < parts) {
-      const float2 ml = triple(base + lane);
-      weight = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-      sum += ml.y * weight;
-    }
-    const int n = min(32, parts - base);
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const float f = __shfl_sync(0xffffffffu, weight, j);
-      const int i = base + j;
-      const float* src = (cut && i >= a.splits ? a.warp_o : a.slab_o) + locate(i) * D + lane * C;
-      if constexpr (C == 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-        if (f != 0.f) {
-          acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
-        }
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-        if (f != 0.f) {
-          acc[0] += f * v.x; acc[1] += f * v.y;
-        }
+    for (int j = 0; j < kMergeBatch; ++j) {
+      const int i = base + j, piece = i - a.splits;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      if (i < parts) {
+        const bool warp_row = cut && piece >= 0;
+        const int64_t at = !warp_row ? (int64_t)i * a.rows + row
+                                     : piece == 0 ? first_row : next_row + (int64_t)(piece - 1) * 2 * a.own_rows;
+        ml[j] = __ldcg((warp_row ? a.warp_ml : a.slab_ml) + at);
+        o[j] = __ldcg(reinterpret_cast<const float4*>((warp_row ? a.warp_o : a.slab_o) + at * D + c));
       }
     }
+    float m = top;
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) m = fmaxf(m, ml[j].x);
+    if (m == -INFINITY) continue;
+    const float f = exp2f(top - m);
+    top = m;
+    sum *= f;
+    acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) {
+      if (ml[j].x == -INFINITY) continue;
+      const float w = exp2f(ml[j].x - m);
+      sum += ml[j].y * w;
+      acc.x += w * o[j].x; acc.y += w * o[j].y; acc.z += w * o[j].z; acc.w += w * o[j].w;
+    }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (p.head_sink) sum += exp2f(sink - top);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* out = static_cast<T*>(p.output) + t * p.output_row_stride + (int64_t)h * D + lane * C;
+  T* out = static_cast<T*>(p.output) + t * p.output_row_stride + (int64_t)h * D + c;
   if (vector_rows) {
-    uint32_t w[C / 2];
-#pragma unroll
-    for (int c = 0; c < C / 2; ++c) w[c] = mma_op<T>::pack(acc[2 * c] * inv, acc[2 * c + 1] * inv);
-    if constexpr (C == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(out) = w[0];
+    *reinterpret_cast<uint2*>(out) = make_uint2(mma_op<T>::pack(acc.x * inv, acc.y * inv), mma_op<T>::pack(acc.z * inv, acc.w * inv));
   } else {
-#pragma unroll
-    for (int c = 0; c < C; ++c) out[c] = act<T>::from_f(acc[c] * inv);
+    out[0] = act<T>::from_f(acc.x * inv);
+    out[1] = act<T>::from_f(acc.y * inv);
+    out[2] = act<T>::from_f(acc.z * inv);
+    out[3] = act<T>::from_f(acc.w * inv);
   }
 }
 
 template <typename T>
 cudaError_t launch_merge_t(const SharedPrefixArgs& a, cudaStream_t stream) {
   const bool vec = (reinterpret_cast<uintptr_t>(a.p.output) | (uintptr_t)(a.p.output_row_stride * 2)) % 8 == 0;
-  const dim3 grid((unsigned)((a.rows + kMergeWarps - 1) / kMergeWarps)), block(32 * kMergeWarps);
+  const int64_t per_cta = kMergeThreads / (a.p.head_size / 4);
+  const dim3 grid((unsigned)((a.rows + per_cta - 1) / per_cta)), block(kMergeThreads);
   return a.p.head_size == 64 ? launch_dependent(shared_prefix_merge_kernel<T, 64>, grid, block, 0, stream, a, (int)vec)
                              : launch_dependent(shared_prefix_merge_kernel<T, 128>, grid, block, 0, stream, a, (int)vec);
 }
@@ -377,7 +366,7 @@ size_t layout(const B200SharedPrefixParams& p, int num_sms, SharedPrefixArgs* a)
   a->next_item = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long)));
   a->seq_tiles = reinterpret_cast<int*>(take(sizeof(int) * ((size_t)p.batch + 1)));
   a->seq_pairs = reinterpret_cast<int*>(take(sizeof(int) * ((size_t)p.batch + 1)));
-  a->token_seq = reinterpret_cast<int*>(take(sizeof(int) * (size_t)p.num_tokens));
+  a->token_info = reinterpret_cast<int4*>(take(sizeof(int4) * (size_t)p.num_tokens));
   a->slab_ml = reinterpret_cast<float2*>(take(sizeof(float2) * slabs * a->rows));
   a->warp_ml = reinterpret_cast<float2*>(take(sizeof(float2) * wrows));
   a->slab_o = reinterpret_cast<float*>(take(sizeof(float) * slabs * a->rows * d));

@@ -2,7 +2,7 @@
 // argument block and programmatic dependent launch.
 //
 // One call is four launches:
-//   shared_prefix_plan_kernel   lengths -> work lists (1 CTA)
+//   shared_prefix_plan_kernel   lengths -> work lists (1 CTA), while the tensor-core pass starts
 //   shared_prefix_tc_kernel     tensor-core pass (tcgen05): every token against a range of the
 //                               prefix's keys, and long chunks against their own keys
 //   shared_prefix_own_kernel    single tokens and short chunks against their own keys (memory bound)
@@ -32,8 +32,9 @@ struct SharedPrefixArgs {
   // plan
   int* seq_tiles;    // [batch + 1] exclusive prefix of 16-key tiles (per kv head), own kernel
   int* seq_pairs;    // [batch + 1] exclusive prefix of query-tile pairs, tensor-core kernel
-  int* token_seq;    // [num_tokens] sequence of a token, -1 without a valid one
-  unsigned long long* next_item;  // tensor-core work list position
+  int4* token_info;  // [num_tokens] of a token's sequence: first token, tokens (-1: none valid), first
+                     // 16-key tile of the own kernel, tiles (0: own keys on the tensor-core kernel)
+  unsigned long long* next_item;  // tensor-core items handed out beyond each CTA's first
   // partials
   float* slab_o;     // [splits + 1][rows][head_size]
   float2* slab_ml;   // [splits + 1][rows]
@@ -48,21 +49,35 @@ struct SharedPrefixMaps {
 
 constexpr int kOwnTile = 16;  // keys per tile of the own kernel
 constexpr int kOwnWarps = 4;  // warps per CTA
-constexpr int kOwnCtasPerSm = 2;  // its shared memory, 97 KB per CTA, leaves room for two
+constexpr int kOwnCtasPerSm = 3;  // its shared memory, 65 KB per CTA, leaves room for three
 constexpr int kPrefixKeys = 128;  // keys per tile of the tensor-core kernel
 
 cudaError_t launch_shared_prefix_tc(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms,
                                     cudaStream_t stream);
 cudaError_t launch_shared_prefix_own(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, cudaStream_t stream);
 
-// Stream-K ranges of the own kernel: warp w of W owns tiles [start(w), start(w + 1)) of T.
-__host__ __device__ __forceinline__ int64_t own_range_start(int64_t w, int64_t T, int64_t W) { return w * T / W; }
-__device__ __forceinline__ int64_t own_warp_of(int64_t x, int64_t T, int64_t W) { return ((x + 1) * W + T - 1) / T - 1; }
-// Warps that share T tiles: all of them, but at least 4 tiles each.
-__device__ __forceinline__ int64_t own_active_warps(int64_t T, int64_t grid_warps) {
-  const int64_t most = (T + 3) / 4;
-  return most < 1 ? 1 : (most < grid_warps ? most : grid_warps);
-}
+// Stream-K ranges of the own kernel: T tiles over W warps, the first `extra` warps own `each` + 1
+// consecutive tiles and the others `each`.
+struct OwnRanges {
+  int64_t total, extra;
+  int64_t each;
+  int64_t warps;
+  __device__ __forceinline__ OwnRanges(int64_t tiles, int grid_warps) : total(tiles) {
+    const int64_t most = (tiles + 1) / 2;  // at least 2 tiles per warp: more pieces cost the merge more
+    warps = most < 1 ? 1 : (most < grid_warps ? most : grid_warps);
+    each = quotient(tiles, warps);
+    extra = tiles - each * warps;
+  }
+  __device__ __forceinline__ int64_t start(int64_t w) const { return w * each + (w < extra ? w : extra); }
+  __device__ __forceinline__ int64_t warp_of(int64_t tile) const {
+    const int64_t split = extra * (each + 1);
+    return tile < split ? quotient(tile, each + 1) : extra + quotient(tile - split, each);
+  }
+  // 32-bit where it fits: a 64-bit division takes several times as long
+  static __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+    return x < (int64_t)1 << 31 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+  }
+};
 
 // Programmatic dependent launch: a kernel launched with the attribute may start once every CTA of
 // the previous one has called release_dependents() (or exited); wait_previous() returns when the

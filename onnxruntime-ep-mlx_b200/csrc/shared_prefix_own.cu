@@ -14,6 +14,8 @@
 // triple per warp, at most two per warp, for the merge kernel.
 #include <atomic>
 
+#include "b200_tcgen05.cuh"
+
 #include "shared_prefix.cuh"
 
 namespace b200 {
@@ -27,7 +29,7 @@ struct OwnLayout {
   static constexpr int kBoxBytes = kOwnTile * 128;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStageBytes = 2 * kTileBytes;  // K and V
-  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kStages = D == 64 ? 4 : 2;
   static constexpr int kSmem = kOwnWarps * kStages * kStageBytes + 1024;
 };
 
@@ -62,11 +64,10 @@ __global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const
 
   const int KV = p.kv_num_heads, g = a.group, H = p.num_heads;
   // The plan is complete: this grid starts after every CTA of the tensor-core kernel has waited for it.
-  const int64_t total_tiles = (int64_t)__ldcg(a.seq_tiles + p.batch) * KV;
-  const int64_t W = own_active_warps(total_tiles, a.own_warps);
+  const OwnRanges ranges((int64_t)__ldcg(a.seq_tiles + p.batch) * KV, a.own_warps);
   const int64_t gw = (int64_t)blockIdx.x * kOwnWarps + warp;
-  const int64_t r0 = gw < W ? own_range_start(gw, total_tiles, W) : 0;
-  const int64_t r1 = gw < W ? own_range_start(gw + 1, total_tiles, W) : 0;
+  const int64_t r0 = gw < ranges.warps ? ranges.start(gw) : 0;
+  const int64_t r1 = gw < ranges.warps ? ranges.start(gw + 1) : 0;
   if (r0 >= r1) {
     wait_previous();  // this grid's completion stands for the tensor-core kernel's, too
     return;
@@ -78,28 +79,50 @@ __global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const
   __syncwarp();
   const float qk_scale = p.softcap > 0.f ? p.scale : p.scale * kLog2e;
 
-  // The piece at stream position x (< r1) into ring slot `slot`.
+  // Sequences seq0 .. seq0 + 31, one per lane, so that going on to the next piece needs no loads.
+  int seq0 = 0, seq_first = 0, seq_c0 = 0, seq_nq = 0, seq_past = 0, seq_tiles = 0;
+  auto load_window = [&](int from) {
+    seq0 = from;
+    const int b = min(from + lane, p.batch);
+    seq_first = __ldcg(a.seq_tiles + b);
+    if (b < p.batch) {
+      seq_tiles = __ldcg(a.seq_tiles + b + 1) - seq_first;
+      seq_c0 = p.cumulative_sequence_length[b];
+      seq_nq = p.cumulative_sequence_length[b + 1] - seq_c0;
+      seq_past = p.past_seqlens[b];
+    }
+  };
+  // The piece at stream position x (< r1) into ring slot `slot` (the whole warp).
   auto locate = [&](int slot, int64_t x) {
     Piece u{};
     if (x < r1) {
-      int lo = 0, hi = p.batch - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((int64_t)__ldcg(a.seq_tiles + mid) * KV <= x) lo = mid; else hi = mid - 1;
+      unsigned before = __ballot_sync(0xffffffffu, (int64_t)seq_first * KV <= x);
+      if (before == 0xffffffffu || before == 0) {  // not in the window: 32-way search
+        int lo = before ? seq0 : 0, hi = p.batch;  // the largest lo with seq_tiles[lo] * KV <= x
+        while (hi - lo > 1) {
+          const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+          const unsigned le = __ballot_sync(0xffffffffu, at < hi && (int64_t)__ldcg(a.seq_tiles + min(at, p.batch)) * KV <= x);
+          lo += (__popc(le) - 1) * step;
+          hi = min(hi, lo + step);
+        }
+        load_window(lo);
+        before = __ballot_sync(0xffffffffu, (int64_t)seq_first * KV <= x);
       }
-      const int first = __ldcg(a.seq_tiles + lo), tiles = __ldcg(a.seq_tiles + lo + 1) - first;
+      // sequences without tiles share their successor's offset: the last one not past x owns it
+      const int src = 31 - __clz(before);
+      const int first = __shfl_sync(0xffffffffu, seq_first, src), tiles = __shfl_sync(0xffffffffu, seq_tiles, src);
+      u.b = seq0 + src;
+      u.c0 = __shfl_sync(0xffffffffu, seq_c0, src);
+      u.nq = __shfl_sync(0xffffffffu, seq_nq, src);
+      u.past = __shfl_sync(0xffffffffu, seq_past, src);
       if (tiles > 0) {
         const int64_t rel = x - (int64_t)first * KV;
         u.valid = 1;
-        u.b = lo;
-        u.kh = (int)(rel / tiles);
+        u.kh = (int)OwnRanges::quotient(rel, tiles);
         u.tiles = tiles;
-        u.t0 = (int)(rel % tiles);
+        u.t0 = (int)(rel - (int64_t)u.kh * tiles);
         u.t1 = (int)min((int64_t)tiles, u.t0 + (r1 - x));
         u.seg_start = (int64_t)first * KV + (int64_t)u.kh * tiles;
-        u.c0 = p.cumulative_sequence_length[lo];
-        u.nq = p.cumulative_sequence_length[lo + 1] - u.c0;
-        u.past = p.past_seqlens[lo];
         u.total = u.past + u.nq;
       }
     }
@@ -130,6 +153,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const
   };
 
   int ps = 0, pt = 0;
+  load_window(0);
   locate(0, r0);
   bool producing = myring[0].valid != 0;
   if (producing) pt = myring[0].t0;
@@ -266,20 +290,26 @@ __global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
           mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
         }
-        const float mn0 = fmaxf(m[n][0], mx0), mn1 = fmaxf(m[n][1], mx1);
-        const float mu0 = mn0 == -INFINITY ? 0.f : mn0, mu1 = mn1 == -INFINITY ? 0.f : mn1;
-        const float al0 = exp2f(m[n][0] - mu0), al1 = exp2f(m[n][1] - mu1);
-        const float p0 = exp2f(sc[0] - mu0), p1 = exp2f(sc[1] - mu1);
-        const float p2 = exp2f(sc[2] - mu0), p3 = exp2f(sc[3] - mu1);
-        l[n][0] = l[n][0] * al0 + p0 + p2;
-        l[n][1] = l[n][1] * al1 + p1 + p3;
-        m[n][0] = mn0;
-        m[n][1] = mn1;
+        // The running maximum moves only when a score exceeds it by more than 2^8 (warp-uniform), so P
+        // stays within 2^8 and most tiles leave o alone.
+        if (__any_sync(0xffffffffu, mx0 > m[n][0] + 8.f || mx1 > m[n][1] + 8.f)) {
+          const float mn0 = fmaxf(m[n][0], mx0), mn1 = fmaxf(m[n][1], mx1);
+          const float al0 = mn0 == -INFINITY ? 1.f : tc::ex2(m[n][0] - mn0), al1 = mn1 == -INFINITY ? 1.f : tc::ex2(m[n][1] - mn1);
+          l[n][0] *= al0;
+          l[n][1] *= al1;
+          m[n][0] = mn0;
+          m[n][1] = mn1;
 #pragma unroll
-        for (int mt = 0; mt < KSTEPS; ++mt) {
-          o[n][mt][0] *= al0; o[n][mt][2] *= al0;
-          o[n][mt][1] *= al1; o[n][mt][3] *= al1;
+          for (int mt = 0; mt < KSTEPS; ++mt) {
+            o[n][mt][0] *= al0; o[n][mt][2] *= al0;
+            o[n][mt][1] *= al1; o[n][mt][3] *= al1;
+          }
         }
+        const float mu0 = m[n][0] == -INFINITY ? 0.f : m[n][0], mu1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+        const float p0 = tc::ex2(sc[0] - mu0), p1 = tc::ex2(sc[1] - mu1);
+        const float p2 = tc::ex2(sc[2] - mu0), p3 = tc::ex2(sc[3] - mu1);
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
         // P to 16 bits twice: the rounded value and what the rounding left (about 16 bits in all)
         const uint32_t x0 = MMA::pack(p0, p1), x1 = MMA::pack(p2, p3);
         const float2 h0 = MMA::unpack(x0), h1 = MMA::unpack(x1);

@@ -15,6 +15,7 @@
 //   warp 9           issues the MMAs: per K/V tile j PV0(j-1), S0(j), PV1(j-1), S1(j), so the tensor
 //                    pipe works on one query tile while the other one's softmax runs
 //   warp 10          loads V tiles
+//   warp 11          lets the own kernel start when the plan is done
 // S = Q K^T (both operands in shared memory), O += P V with P in tensor memory over S's columns (fp16:
 // one value per key; bf16: a hi + lo pair, since one bf16 P costs up to 3e-3 on unit-scale values)
 // and V as the MN-major operand in the cache's [key][channel] order.  The running maximum moves, and
@@ -195,10 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  wait_previous();       // the plan
-  release_dependents();  // the own kernel needs the plan, not this kernel
   const int64_t prefix_items = (int64_t)a.splits * p.kv_num_heads * a.query_pairs;
-  const int64_t n_items = prefix_items + (int64_t)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads;
 
   auto wait_idx = [&](uint64_t* bar, uint32_t index) -> bool {  // completion `index` of a barrier
     if (s_failed) return false;
@@ -210,12 +208,20 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
   auto wait_warp = [&](uint64_t* bar, uint32_t index) -> bool { return __all_sync(0xffffffffu, wait_idx(bar, index)); };
   auto failed_warp = [&]() -> bool { return __any_sync(0xffffffffu, s_failed != 0); };
   auto drain_idx = [&](uint64_t* bar, uint32_t index) { mbar_wait(bar, index & 1u); };
+  // Warp 8 hands out the CTA's k-th item (-1: no more).  The first is the CTA's own and, if it lies in
+  // the prefix, needs nothing of the plan, which may still be running then.
   auto fetch_item = [&](uint32_t k, int64_t& it) -> bool {
     const uint32_t slot = k % kSched;
     if (k >= (uint32_t)kSched && !wait_warp(&bars.sched_empty[slot], k / kSched - 1)) return false;
-    long long v = 0;
+    long long v = blockIdx.x;
+    if (k > 0 || v >= prefix_items) {
+      wait_previous();
+      if (lane == 0) {
+        if (k > 0) v = (long long)gridDim.x + (long long)atomicAdd(a.next_item, 1ull);
+        if (v >= prefix_items + (long long)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads) v = -1;
+      }
+    }
     if (lane == 0) {
-      v = (long long)atomicAdd(a.next_item, 1ull);
       s_item[slot] = v;
       mbar_arrive(&bars.sched_full[slot]);
     }
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
       bool ok = true;
       for (uint32_t k = 0; ok && !failed_warp(); ++k) {
         int64_t it;
-        if (!(ok = is_v ? take_item(k, it) : fetch_item(k, it)) || it >= n_items) break;
+        if (!(ok = is_v ? take_item(k, it) : fetch_item(k, it)) || it < 0) break;
         const Item m = decode_item(a, it, prefix_items);
         if (!is_v) {
           for (int w = 0; w < 2 && ok; ++w) {
@@ -306,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
       bool issued = false, ok = true;
       for (uint32_t k = 0; ok && !failed_warp(); ++k) {
         int64_t it;
-        if (!(ok = take_item(k, it)) || it >= n_items) break;
+        if (!(ok = take_item(k, it)) || it < 0) break;
         const Item m = decode_item(a, it, prefix_items);
 #pragma unroll 1
         for (int j = 0; j <= m.n && ok; ++j) {
@@ -367,6 +373,10 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
         drain_idx(&bars.drain, 0);
       }
       __syncwarp();
+    } else {
+      // The own kernel needs the plan, not this kernel's results: let it start once the plan is done.
+      wait_previous();
+      release_dependents();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -379,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
     uint32_t t = 0, items = 0;
     for (uint32_t k = 0; !failed_warp(); ++k) {
       int64_t it;
-      if (!take_item(k, it) || it >= n_items) break;
+      if (!take_item(k, it) || it < 0) break;
       const Item m = decode_item(a, it, prefix_items);
       const int nw = tiles_of(m, w);
       if (nw == 0) continue;
