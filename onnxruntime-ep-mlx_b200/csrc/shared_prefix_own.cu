@@ -29,8 +29,8 @@ struct OwnLayout {
   static constexpr int kBoxBytes = kOwnTile * 128;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStageBytes = 2 * kTileBytes;  // K and V
-  static constexpr int kStages = D == 64 ? 4 : 2;
-  static constexpr int kSmem = kOwnWarps * kStages * kStageBytes + 1024;
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kSmem = kOwnWarps * kStages * kStageBytes;
 };
 
 // 16-byte piece `chunk` of tile row `row` in the 128B-swizzled boxes.
@@ -45,18 +45,17 @@ struct Piece {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const __grid_constant__ SharedPrefixArgs a,
+__global__ void __launch_bounds__(32 * kOwnWarps, NT == 1 ? 4 : 3) shared_prefix_own_kernel(const __grid_constant__ SharedPrefixArgs a,
                                                                             const __grid_constant__ SharedPrefixMaps maps) {
   using L = OwnLayout<D>;
   using MMA = mma_op<T>;
   constexpr int KSTEPS = D / 16, STAGES = L::kStages, RING = STAGES + 1, ROWS = 8 * NT;
-  extern __shared__ uint8_t dyn_smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kOwnWarps][STAGES];
   __shared__ Piece ring[kOwnWarps][RING];
 
   release_dependents();
   const B200SharedPrefixParams& p = a.p;
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* wbase = smem + warp * STAGES * L::kStageBytes;
   const uint32_t wbase_u32 = smem_u32(wbase);
@@ -69,7 +68,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const
   const int64_t r0 = gw < ranges.warps ? ranges.start(gw) : 0;
   const int64_t r1 = gw < ranges.warps ? ranges.start(gw + 1) : 0;
   if (r0 >= r1) {
-    wait_previous();  // this grid's completion stands for the tensor-core kernel's, too
+    if (blockIdx.x == gridDim.x - 1) wait_previous();  // as at the end
     return;
   }
   if (lane == 0) {
@@ -370,7 +369,9 @@ __global__ void __launch_bounds__(32 * kOwnWarps) shared_prefix_own_kernel(const
     cs = (cs + 1) % RING;
     ct = myring[cs].t0;
   }
-  wait_previous();  // this grid's completion stands for the tensor-core kernel's, too
+  // The last CTA stays until the tensor-core kernel is done: the merge, which waits for this grid, then
+  // has both.  The others leave their place to this grid's next CTAs.
+  if (blockIdx.x == gridDim.x - 1) wait_previous();
 }
 
 template <typename T, int D, int NT>
@@ -382,6 +383,9 @@ cudaError_t launch_own_t(const SharedPrefixArgs& a, const SharedPrefixMaps& maps
   if (e != cudaSuccess) return e;
   if (!ready[dev & 63].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnLayout<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    // both kernels' CTAs share an SM only in the largest shared-memory split
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
     ready[dev & 63].store(1, std::memory_order_release);
   }

@@ -44,20 +44,23 @@ template <int D>
 struct TcLayout {
   static constexpr int kBoxes = D / 64;
   static constexpr int kTile = kBoxes * kBoxBytes;
-  static constexpr int kKStages = D == 64 ? 4 : 2;
-  static constexpr int kVStages = D == 64 ? 4 : 3;
+  static constexpr int kKStages = D == 64 ? 4 : 1;
+  static constexpr int kVStages = D == 64 ? 4 : 2;
   static constexpr int kSmemQ = 0;
   static constexpr int kSmemK = 2 * kTile;
   static constexpr int kSmemV = kSmemK + kKStages * kTile;
-  static constexpr int kSmem = kSmemV + kVStages * kTile + 1024;
+  static constexpr int kSmem = kSmemV + kVStages * kTile;  // 160 KB: the own kernel's CTA fits beside it
 };
 
 constexpr int kWg = 128;
 constexpr int kThreads = 3 * kWg;
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kVLoadWarp = 10;
-constexpr int kSoftmaxRegs = 200, kControlRegs = 96;  // setmaxnreg split
+// Registers: launched with 128 per thread (the launch bound of 512 threads sets that), which leaves
+// the register file room for a CTA of the own kernel; setmaxnreg then splits them.
+constexpr int kBoundThreads = 512;
+constexpr int kSoftmaxRegs = 152, kControlRegs = 80;
 constexpr int kSplitRegs = 2 * kWg * kSoftmaxRegs + kWg * kControlRegs;
-static_assert(kSplitRegs <= kThreads * 168, "the register split exceeds the launch allocation");
+static_assert(kSplitRegs <= kThreads * 128, "the register split exceeds the launch allocation");
 constexpr int kSched = 4;  // slots of the item queue
 constexpr int kTakers = 2 * kWg / 32 + 2;
 
@@ -148,7 +151,7 @@ __device__ __noinline__ void fill_tail_page(uint8_t* stage, const B200SharedPref
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __grid_constant__ SharedPrefixArgs a,
+__global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(const __grid_constant__ SharedPrefixArgs a,
                                                                         const __grid_constant__ SharedPrefixMaps maps) {
   using L = TcLayout<D>;
   using MMA = mma_op<T>;
@@ -157,14 +160,13 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
   constexpr uint32_t kIdPV = tc::idesc_f16(kBM, D, kBF16, false, true);
   constexpr int kKStages = L::kKStages, kVStages = L::kVStages;
 
-  extern __shared__ uint8_t dyn_smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) Bars bars;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int s_failed;
   __shared__ volatile long long s_item[kSched];
 
   const B200SharedPrefixParams& p = a.p;
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = a.group, H = p.num_heads, TQ = a.tile_tokens;
@@ -410,14 +412,18 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_tc_kernel(const __g
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx[r] = -INFINITY;
         if (raw) {
-          float sv[kBN / 32][32];
 #pragma unroll
-          for (int c = 0; c < kBN / 32; ++c) tc::ld32(sbuf + c * 32, sv[c]);
-          tc::wait_ld();
+          for (int c = 0; c < kBN / 32; c += 2) {
+            float xa[32], xb[32];
+            tc::ld32(sbuf + c * 32, xa);
+            tc::ld32(sbuf + (c + 1) * 32, xb);
+            tc::wait_ld();
 #pragma unroll
-          for (int c = 0; c < kBN / 32; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx[i & 3] = tc::max3(mx[i & 3], sv[c][2 * i], sv[c][2 * i + 1]);
+            for (int i = 0; i < 16; ++i) {
+              mx[i & 3] = tc::max3(mx[i & 3], xa[2 * i], xa[2 * i + 1]);
+              mx[i & 3] = tc::max3(mx[i & 3], xb[2 * i], xb[2 * i + 1]);
+            }
+          }
         } else {
           const int vhi = last - kbase;
 #pragma unroll 1
@@ -544,6 +550,9 @@ cudaError_t launch_tc_t(const SharedPrefixArgs& a, const SharedPrefixMaps& maps,
   static std::atomic<uint32_t> ready[64];  // per device: attributes set and checked
   if (!ready[dev & 63].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    // both kernels' CTAs share an SM only in the largest shared-memory split
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
     cudaFuncAttributes attr;  // setmaxnreg.inc waits until the launch allocation covers the split
     e = cudaFuncGetAttributes(&attr, kernel);
