@@ -23,6 +23,14 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// 16 bytes global -> shared memory, or 16 zero bytes.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 template <int D>
 struct OwnLayout {
   static constexpr int kBoxes = D / 64;
@@ -51,14 +59,12 @@ __global__ void __launch_bounds__(32 * kOwnWarps, NT == 1 ? 4 : 3) shared_prefix
   using MMA = mma_op<T>;
   constexpr int KSTEPS = D / 16, STAGES = L::kStages, RING = STAGES + 1, ROWS = 8 * NT;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[kOwnWarps][STAGES];
   __shared__ Piece ring[kOwnWarps][RING];
 
   release_dependents();
   const B200SharedPrefixParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* wbase = smem + warp * STAGES * L::kStageBytes;
-  const uint32_t wbase_u32 = smem_u32(wbase);
+  const uint32_t wbase_u32 = smem_u32(smem + warp * STAGES * L::kStageBytes);
   Piece* myring = ring[warp];
 
   const int KV = p.kv_num_heads, g = a.group, H = p.num_heads;
@@ -71,11 +77,6 @@ __global__ void __launch_bounds__(32 * kOwnWarps, NT == 1 ? 4 : 3) shared_prefix
     if (blockIdx.x == gridDim.x - 1) wait_previous();  // as at the end
     return;
   }
-  if (lane == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&bars[warp][s], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
   const float qk_scale = p.softcap > 0.f ? p.scale : p.scale * kLog2e;
 
   // Sequences seq0 .. seq0 + 31, one per lane, so that going on to the next piece needs no loads.
@@ -130,57 +131,65 @@ __global__ void __launch_bounds__(32 * kOwnWarps, NT == 1 ? 4 : 3) shared_prefix
     __syncwarp();
   };
 
-  auto issue = [&](int s, int slot, int t) {  // lane 0: the TMA loads of tile t into stage s
-    if (lane != 0) return;
-    const Piece& u = myring[slot];
-    uint64_t* bar = &bars[warp][s];
-    const int pos = t * kOwnTile;
-    const int32_t blk = p.block_table[(int64_t)u.b * p.max_blocks_per_seq + pos / p.block_size];
-    if (blk < 0 || blk >= p.num_blocks) {
-      set_status(p.device_status, kStatusBadBlock);
-      mbar_arrive(bar);
-      return;
-    }
-    const int z = blk * p.block_size + pos % p.block_size;
-    uint8_t* kdst = wbase + s * L::kStageBytes;
-    mbar_arrive_expect_tx(bar, L::kStageBytes);
-#pragma unroll
-    for (int h = 0; h < L::kBoxes; ++h) {
-      tma_load_3d(kdst + h * L::kBoxBytes, &maps.k_map, bar, h * 64, u.kh, z);
-      tma_load_3d(kdst + L::kTileBytes + h * L::kBoxBytes, &maps.v_map, bar, h * 64, u.kh, z);
-    }
-  };
-
-  int ps = 0, pt = 0;
-  load_window(0);
-  locate(0, r0);
-  bool producing = myring[0].valid != 0;
-  if (producing) pt = myring[0].t0;
-  uint32_t phase = 0, pending = 0;
-  int issued = 0, consumed = 0;
-  bool failed = false;
+  // Producer: tile pt of the piece in ring slot ps goes into stage `issued` % STAGES, 16 bytes per lane
+  // and copy; rows without a key (past the sequence's end, or of a block id out of range) become zeros.
+  const char* const kv_base[2] = {static_cast<const char*>(p.key_cache), static_cast<const char*>(p.value_cache)};
+  const int64_t row_bytes = (int64_t)KV * D * 2;
+  int ps = 0, pt = 0, issued = 0, window = 0;
+  int32_t window_blk = -1;  // lane i: block of tile window + i of the piece
+  bool producing = false, fresh = true;
   auto produce = [&]() {
     while (producing && pt >= myring[ps].t1) {
       const int64_t next = myring[ps].seg_start + myring[ps].t1;
       ps = (ps + 1) % RING;
       locate(ps, next);
       producing = myring[ps].valid != 0;
-      if (producing) pt = myring[ps].t0;
+      pt = myring[ps].t0;
+      fresh = true;
     }
-    if (!producing) return;
-    const int s = issued % STAGES;
-    issue(s, ps, pt);
-    pending |= 1u << s;
-    ++pt;
-    ++issued;
+    if (producing) {
+      const Piece& u = myring[ps];
+      if (fresh || pt - window == 32) {
+        fresh = false;
+        window = pt;
+        window_blk = pt + lane < u.t1 ? __ldg(p.block_table + (int64_t)u.b * p.max_blocks_per_seq +
+                                              (pt + lane) * kOwnTile / p.block_size)
+                                      : -1;
+      }
+      const int32_t blk = __shfl_sync(0xffffffffu, window_blk, pt - window);
+      const int pos = pt * kOwnTile;
+      const bool ok = blk >= 0 && blk < p.num_blocks;
+      if (!ok && lane == 0) set_status(p.device_status, kStatusBadBlock);
+      const int keys = ok ? u.total - pos : 0;
+      const int64_t first = ok ? (((int64_t)blk * p.block_size + pos % p.block_size) * KV + u.kh) * D * 2 : 0;
+      const uint32_t dst = wbase_u32 + issued % STAGES * L::kStageBytes;
+      constexpr int CH = D / 8;  // 16-byte pieces per row
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const char* src = kv_base[t] + first + lane / CH * row_bytes + lane % CH * 16;
+#pragma unroll
+        for (int i = 0; i < kOwnTile * CH / 32; ++i) {
+          const int row = i * (32 / CH) + lane / CH;
+          cp_async16(dst + t * L::kTileBytes + own_swizzle(row, lane % CH), row < keys ? src : kv_base[t], row < keys);
+          src += 32 / CH * row_bytes;
+        }
+      }
+      ++pt;
+      ++issued;
+    }
+    cp_async_commit();  // a group per call, empty at the end
   };
+  load_window(0);
+  locate(0, r0);
+  producing = myring[0].valid != 0;
+  pt = myring[0].t0;
+  int consumed = 0;
   for (int i = 0; i < STAGES; ++i) produce();
-  __syncwarp();
 
   int cs = 0, ct = myring[0].t0;
   const int col0 = (lane & 3) * 2;  // rows held by this lane: 8 n + col0, + 1
 
-  while (consumed < issued && !failed) {
+  while (consumed < issued) {
     const Piece u = myring[cs];
     const int rows = u.nq * g;
 
@@ -212,45 +221,14 @@ __global__ void __launch_bounds__(32 * kOwnWarps, NT == 1 ? 4 : 3) shared_prefix
 #pragma unroll
       for (int mt = 0; mt < KSTEPS; ++mt) o[n][mt][0] = o[n][mt][1] = o[n][mt][2] = o[n][mt][3] = 0.f;
     }
-    // block ids of 32 tiles at a time: lane i holds tile wb + i's, the next window loaded ahead
-    auto tile_block = [&](int t) -> int32_t {
-      return t < u.t1 ? __ldg(p.block_table + (int64_t)u.b * p.max_blocks_per_seq + t * kOwnTile / p.block_size) : -1;
-    };
-    int wb = ct;
-    int32_t w_blk = tile_block(wb + lane), n_blk = -1;
 
     for (; ct < u.t1; ++ct) {
       const int s = consumed % STAGES;
       const int pos0 = ct * kOwnTile;
-      int wi = ct - wb;
-      if (wi == 32) {
-        wb = ct;
-        wi = 0;
-        w_blk = n_blk;
-      }
-      if (wi == 0) n_blk = tile_block(wb + 32 + lane);
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars[warp][s], (phase >> s) & 1u))) {
-        if (lane == 0) set_status(p.device_status, kStatusTimeout);
-        failed = true;
-        for (int s2 = 0; s2 < STAGES; ++s2)  // one more bounded wait for the loads in flight
-          if ((pending >> s2) & 1u) mbar_wait(&bars[warp][s2], (phase >> s2) & 1u);
-        break;
-      }
-      phase ^= 1u << s;
-      pending &= ~(1u << s);
-      const int32_t blk = __shfl_sync(0xffffffffu, w_blk, wi);
-      const bool blk_ok = blk >= 0 && blk < p.num_blocks;
-      const bool full = blk_ok && pos0 + kOwnTile <= u.past + 1;  // every row sees every key
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
+      const bool full = pos0 + kOwnTile <= u.past + 1;  // every row sees every key
       const uint32_t kbase = wbase_u32 + s * L::kStageBytes, vbase = kbase + L::kTileBytes;
-      const bool tail = pos0 + kOwnTile > u.total;
-      if (tail || !blk_ok) {
-        // V rows of unused slots become zeros: 0 x NaN from whatever they hold would poison o
-        const int first = blk_ok ? u.total - pos0 : 0;
-        for (int i = lane; i < (kOwnTile - first) * (D / 8); i += 32)
-          *reinterpret_cast<uint4*>(wbase + (vbase - wbase_u32) + own_swizzle(first + i / (D / 8), i % (D / 8))) =
-              make_uint4(0u, 0u, 0u, 0u);
-        __syncwarp();
-      }
 
       float c[NT][2][4];
 #pragma unroll
@@ -280,7 +258,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, NT == 1 ? 4 : 3) shared_prefix
           const int pos = pos0 + (lane >> 2) + ((e >> 1) << 3);
           float x = (c[n][0][e] + c[n][1][e]) * qk_scale;
           if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap) * kLog2e;
-          const bool seen = full ? limit[n][e & 1] >= 0 : blk_ok && pos <= limit[n][e & 1];
+          const bool seen = full ? limit[n][e & 1] >= 0 : pos <= limit[n][e & 1];
           sc[e] = seen ? x : -INFINITY;
         }
         float mx0 = fmaxf(sc[0], sc[2]), mx1 = fmaxf(sc[1], sc[3]);
@@ -332,13 +310,9 @@ __global__ void __launch_bounds__(32 * kOwnWarps, NT == 1 ? 4 : 3) shared_prefix
         }
       }
       __syncwarp();
-      if (tail || !blk_ok) fence_proxy_async_smem();  // the zeros before the next TMA write
-      __syncwarp();
       ++consumed;
       produce();
-      __syncwarp();
     }
-    if (failed) break;
 
     // the piece's triples: column sums of l, then the own slab or this warp's rows
     const int dr = lane >> 2;
