@@ -121,7 +121,11 @@ void launch_generic_t(const B200SharedPrefixParams& p, cudaStream_t stream) {
 
 
 // ---------------------------------------------------------------------------------------------
-// Plan: one CTA checks the lengths, routes every sequence and lays out both work lists.
+// Plan: CTA 0 checks the lengths, routes every sequence and lays out both work lists.  The other CTAs,
+// where launched, copy the prefix's bf16 values to fp16 [key][kv head][channel]: with fp16 values the
+// tensor-core pass can carry P as one fp16 value instead of a bf16 hi + lo pair, which takes a third of
+// its MMA work.  The conversion is exact from 2^-14 up to 65504 (below, within 2^-25); a CTA that meets
+// anything beyond, or a NaN, says so and the tensor-core pass then reads the bf16 pages.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
@@ -160,10 +164,37 @@ __device__ __forceinline__ int2 block_inclusive_sum(int2 v, int2* warp_sums, int
   return v;
 }
 
+__device__ __forceinline__ void copy_prefix_values(const SharedPrefixArgs& a) {
+  const B200SharedPrefixParams& p = a.p;
+  const int64_t vecs = (int64_t)p.kv_num_heads * p.head_size / 8;  // 16-byte pieces of one key's values
+  const int64_t n = vecs * p.prefix_length, step = (int64_t)a.copy_ctas * kPlanThreads;
+  uint32_t over = 0;
+#pragma unroll 4
+  for (int64_t i = (int64_t)(blockIdx.x - 1) * kPlanThreads + threadIdx.x; i < n; i += step) {
+    const int64_t key = i / vecs;
+    const int32_t blk = __ldg(p.prefix_block_table + key / p.block_size);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (blk >= 0 && blk < p.num_blocks)  // the tensor-core kernel reports the others
+      v = __ldg(static_cast<const uint4*>(p.value_cache) + ((int64_t)blk * p.block_size + key % p.block_size) * vecs + (i - key * vecs));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      over |= (w[k] & 0x7fff7fffu) + 0x38803880u;  // bit 15 / 31: bf16 magnitude 0x4780 (65536) and above
+      const __half2 h = __floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+      o[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    reinterpret_cast<uint4*>(a.v_copy)[i] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  const int wide = __syncthreads_or((over & 0x80008000u) != 0);
+  if (threadIdx.x == 0) a.v_wide[blockIdx.x - 1] = wide;
+}
+
 __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const SharedPrefixArgs a) {
   __shared__ int2 warp_sums[32];
   const B200SharedPrefixParams& p = a.p;
   release_dependents();
+  if (blockIdx.x > 0) return copy_prefix_values(a);
   const int tid = threadIdx.x, lane = tid & 31;
   for (int t = tid; t < p.num_tokens; t += kPlanThreads) a.token_info[t] = make_int4(0, -1, 0, 0);
   if (tid == 0) *a.next_item = 0;
@@ -309,6 +340,12 @@ cudaError_t launch_merge_t(const SharedPrefixArgs& a, cudaStream_t stream) {
 // ---------------------------------------------------------------------------------------------
 // Host side of the fast path
 // ---------------------------------------------------------------------------------------------
+// Pairs of query tiles up to which head size 128 shares the SMs with the own kernel.  Whole calls shared and
+// not (8192 keys, 8 kv heads): 1 pair 49 against 55 us, 2 pairs 94 against 105, 4 pairs 118 against 120, 8
+// pairs 209 against 201.  Head size 64 gives up nothing for it and always shares.
+constexpr int kBesidePairs = 4;
+constexpr int kCopyPairs = 4;  // pairs of query tiles from which the copy of the prefix's values pays
+
 // The shapes the fast path covers; the call also needs 16-byte rows (fast_rows).
 bool fast_shape(const B200SharedPrefixParams& p) {
   return (p.head_size == 64 || p.head_size == 128) && p.block_size % kOwnTile == 0 &&
@@ -355,6 +392,12 @@ size_t layout(const B200SharedPrefixParams& p, int num_sms, SharedPrefixArgs* a)
   a->own_warps = num_sms * kOwnCtasPerSm * kOwnWarps;
   a->rows = (int64_t)p.num_tokens * p.num_heads;
   split_prefix(a, num_sms);
+  // The copy of the values costs about 4 bytes per value once, and saves every pair of query tiles a
+  // third of its MMA work on them.  Whole calls with and without it (8192 keys, 8 kv heads, d 128 / 64):
+  // 1 pair 56 / 41 against 55 / 39 us, 4 pairs 119 / 85 against 118 / 91, 8 pairs 201 / 152 against 209 / 164.
+  const bool copy = p.act_dtype == B200_DTYPE_BFLOAT16 && p.prefix_length > 0 && a->query_pairs >= kCopyPairs;
+  a->beside = p.head_size == 64 || a->query_pairs <= kBesidePairs;
+  a->copy_ctas = copy ? 2 * num_sms - 1 : 0;
   char* base = static_cast<char*>(p.workspace);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -371,6 +414,11 @@ size_t layout(const B200SharedPrefixParams& p, int num_sms, SharedPrefixArgs* a)
   a->warp_ml = reinterpret_cast<float2*>(take(sizeof(float2) * wrows));
   a->slab_o = reinterpret_cast<float*>(take(sizeof(float) * slabs * a->rows * d));
   a->warp_o = reinterpret_cast<float*>(take(sizeof(float) * wrows * d));
+  a->v_copy = nullptr;
+  if (copy) {
+    a->v_wide = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * a->copy_ctas));
+    a->v_copy = reinterpret_cast<__half*>(take(2 * (size_t)p.prefix_length * p.kv_num_heads * d));
+  }
   return off;
 }
 
@@ -387,6 +435,11 @@ cudaError_t encode_maps(const SharedPrefixArgs& a, SharedPrefixMaps* maps) {
       encode_tensor_map(&maps->v_map, bf, 3, p.value_cache, dims, strides, box) ||
       encode_tensor_map(&maps->q_map, bf, 3, p.query, q_dims, q_strides, q_box))
     return cudaErrorInvalidValue;
+  if (a.v_copy) {
+    const uint64_t c_dims[3] = {d, kv, (uint64_t)p.prefix_length};
+    const uint32_t c_box[3] = {64, 1, kPrefixKeys};
+    if (encode_tensor_map(&maps->vc_map, false, 3, a.v_copy, c_dims, strides, c_box)) return cudaErrorInvalidValue;
+  }
   return cudaSuccess;
 }
 
@@ -405,10 +458,10 @@ cudaError_t launch_shared_prefix(const B200SharedPrefixParams& p, int num_sms, c
     add_launches(1);
     return cudaGetLastError();
   }
-  SharedPrefixMaps maps;
+  SharedPrefixMaps maps{};
   cudaError_t e = encode_maps(a, &maps);
   if (e != cudaSuccess) return e;
-  shared_prefix_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+  shared_prefix_plan_kernel<<<1 + a.copy_ctas, kPlanThreads, 0, stream>>>(a);
   e = cudaGetLastError();
   if (e == cudaSuccess) e = launch_shared_prefix_tc(a, maps, num_sms, stream);
   if (e == cudaSuccess) e = launch_shared_prefix_own(a, maps, stream);

@@ -29,6 +29,11 @@ struct SharedPrefixArgs {
   int own_rows;      // sequences of at most this many (token, head-in-group) rows: own kernel
   int own_warps;     // warps of the own kernel's grid
   int64_t rows;      // num_tokens * num_heads
+  int beside;        // tensor-core CTAs leave room for the own kernel's
+  // fp16 copy of the prefix's values (bf16 calls whose copy pays: see shared_prefix_plan_kernel)
+  __half* v_copy;    // [prefix_length][kv heads][head_size], or null
+  uint32_t* v_wide;  // [copy_ctas] nonzero: the CTA met a value beyond the fp16 range
+  int copy_ctas;
   // plan
   int* seq_tiles;    // [batch + 1] exclusive prefix of 16-key tiles (per kv head), own kernel
   int* seq_pairs;    // [batch + 1] exclusive prefix of query-tile pairs, tensor-core kernel
@@ -45,6 +50,7 @@ struct SharedPrefixArgs {
 struct SharedPrefixMaps {
   CUtensorMap k_map, v_map;  // [num_blocks * block_size, kv heads, d]: box {64, 1, 16}
   CUtensorMap q_map;         // [tokens, heads, d]: box {64, group, tile_tokens}
+  CUtensorMap vc_map;        // v_copy: box {64, 1, 128}
 };
 
 constexpr int kOwnTile = 16;  // keys per tile of the own kernel

@@ -16,9 +16,10 @@
 //                    pipe works on one query tile while the other one's softmax runs
 //   warp 10          loads V tiles
 //   warp 11          lets the own kernel start when the plan is done
-// S = Q K^T (both operands in shared memory), O += P V with P in tensor memory over S's columns (fp16:
-// one value per key; bf16: a hi + lo pair, since one bf16 P costs up to 3e-3 on unit-scale values)
-// and V as the MN-major operand in the cache's [key][channel] order.  The running maximum moves, and
+// S = Q K^T (both operands in shared memory), O += P V with P in tensor memory over S's columns and V as
+// the MN-major operand in the cache's [key][channel] order.  P is one fp16 value per key against fp16
+// values (fp16 calls, or bf16 calls on the plan's fp16 copy of the prefix's values) and a hi + lo pair
+// of bf16 values against bf16 ones, since one bf16 P costs up to 3e-3 on unit-scale values.  The running maximum moves, and
 // O is rescaled, only when it grows by more than 2^8.  Tensor memory: S/P 0 and 1 at columns 0 and
 // 128, O 0 and 1 at 256 and 384.  Each item leaves its rows' (m, l, o) in a slab.
 // Every wait is bounded; one that runs out sets the status word, the roles drain what they issued,
@@ -40,27 +41,31 @@ constexpr int kBoxBytes = 128 * 128;  // [128 rows][64 channels]
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPolyEvery = 4;       // every 4th exponential pair on the FMA pipe
 
-template <int D>
+// Two shapes of the kernel.  BESIDE: 160 KB of shared memory and 128 registers per thread at launch (its
+// launch bound of 512 threads sets that), so a CTA of the own kernel fits on the SM beside it; for head
+// size 128 that leaves one K stage, whose next tile arrives about 900 cycles late.  Otherwise (head size
+// 128 only) the SM is this kernel's alone.
+template <int D, bool BESIDE>
 struct TcLayout {
   static constexpr int kBoxes = D / 64;
   static constexpr int kTile = kBoxes * kBoxBytes;
-  static constexpr int kKStages = D == 64 ? 4 : 1;
-  static constexpr int kVStages = D == 64 ? 4 : 2;
+  static constexpr int kKStages = D == 64 ? 4 : BESIDE ? 1 : 2;
+  static constexpr int kVStages = D == 64 ? 4 : BESIDE ? 2 : 3;
   static constexpr int kSmemQ = 0;
   static constexpr int kSmemK = 2 * kTile;
   static constexpr int kSmemV = kSmemK + kKStages * kTile;
-  static constexpr int kSmem = kSmemV + kVStages * kTile;  // 160 KB: the own kernel's CTA fits beside it
+  static constexpr int kSmem = kSmemV + kVStages * kTile;
+  // setmaxnreg split of the registers per thread at launch
+  static constexpr int kBoundThreads = BESIDE ? 512 : 384;
+  static constexpr int kLaunchRegs = BESIDE ? 128 : 168;
+  static constexpr int kSoftmaxRegs = BESIDE ? 152 : 200, kControlRegs = BESIDE ? 80 : 96;
+  static constexpr int kSplitRegs = 2 * 128 * kSoftmaxRegs + 128 * kControlRegs;
+  static_assert(kSplitRegs <= 384 * kLaunchRegs, "the register split exceeds the launch allocation");
 };
 
 constexpr int kWg = 128;
 constexpr int kThreads = 3 * kWg;
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kVLoadWarp = 10;
-// Registers: launched with 128 per thread (the launch bound of 512 threads sets that), which leaves
-// the register file room for a CTA of the own kernel; setmaxnreg then splits them.
-constexpr int kBoundThreads = 512;
-constexpr int kSoftmaxRegs = 152, kControlRegs = 80;
-constexpr int kSplitRegs = 2 * kWg * kSoftmaxRegs + kWg * kControlRegs;
-static_assert(kSplitRegs <= kThreads * 128, "the register split exceeds the launch allocation");
 constexpr int kSched = 4;  // slots of the item queue
 constexpr int kTakers = 2 * kWg / 32 + 2;
 
@@ -68,7 +73,7 @@ struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t s_full[2], p_full[2], o_done[2];
-  uint64_t drain;
+  uint64_t drain, plan;
   uint64_t sched_full[kSched], sched_empty[kSched];
 };
 
@@ -150,20 +155,20 @@ __device__ __noinline__ void fill_tail_page(uint8_t* stage, const B200SharedPref
   __syncwarp();
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(const __grid_constant__ SharedPrefixArgs a,
+template <typename T, int D, bool BESIDE>
+__global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) shared_prefix_tc_kernel(const __grid_constant__ SharedPrefixArgs a,
                                                                         const __grid_constant__ SharedPrefixMaps maps) {
-  using L = TcLayout<D>;
+  using L = TcLayout<D, BESIDE>;
   using MMA = mma_op<T>;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdQK = tc::idesc_f16(kBM, kBN, kBF16, false, false);
-  constexpr uint32_t kIdPV = tc::idesc_f16(kBM, D, kBF16, false, true);
+  constexpr uint32_t kIdPV = tc::idesc_f16(kBM, D, kBF16, false, true), kIdPV16 = tc::idesc_f16(kBM, D, false, false, true);
   constexpr int kKStages = L::kKStages, kVStages = L::kVStages;
 
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) Bars bars;
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int s_failed;
+  __shared__ volatile int s_failed, s_copy;  // s_copy: prefix items take the values' fp16 copy
   __shared__ volatile long long s_item[kSched];
 
   const B200SharedPrefixParams& p = a.p;
@@ -187,6 +192,7 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
       mbar_init(&bars.v_empty[i], 1);
     }
     mbar_init(&bars.drain, 1);
+    mbar_init(&bars.plan, 1);
     for (int i = 0; i < kSched; ++i) {
       mbar_init(&bars.sched_full[i], 1);
       mbar_init(&bars.sched_empty[i], kTakers);
@@ -239,8 +245,20 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
     return true;
   };
 
+  // Whether an item's values come from the fp16 copy; waits for the plan (which decides it) at the first
+  // prefix item of a call that made the copy.
+  bool plan_seen = false;
+  auto takes_copy = [&](const Item& m, bool& copy) -> bool {
+    copy = false;
+    if (!a.v_copy || m.chunk) return true;
+    if (!plan_seen && !wait_warp(&bars.plan, 0)) return false;
+    plan_seen = true;
+    copy = s_copy != 0;
+    return true;
+  };
+
   if (warp >= 2 * (kWg / 32)) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kControlRegs));
     if (warp == kLoadWarp || warp == kVLoadWarp) {
       // ---------------------------------------------------------------- TMA producers
       const bool is_v = warp == kVLoadWarp;
@@ -259,6 +277,8 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
         int64_t it;
         if (!(ok = is_v ? take_item(k, it) : fetch_item(k, it)) || it < 0) break;
         const Item m = decode_item(a, it, prefix_items);
+        bool copied = false;
+        if (is_v && !(ok = takes_copy(m, copied))) break;
         if (!is_v) {
           for (int w = 0; w < 2 && ok; ++w) {
             if (tiles_of(m, w) == 0) continue;
@@ -276,6 +296,18 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
           const int pos = m.k_lo + j * kBN + page * kPage;
           return loader && pos < m.k_valid ? __ldg(m.table + pos / p.block_size) : -1;
         };
+        if (copied) {  // contiguous rows; TMA fills zeros past the last key
+          for (int j = 0; j < m.n && ok; ++j, ++c) {
+            const uint32_t st = c % stages;
+            if (c >= stages && !(ok = wait_warp(&empty_bar[st], c / stages - 1))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], L::kTile);
+            __syncwarp();
+            if (lane < L::kBoxes)
+              tma_load_3d(smem + ring + st * L::kTile + lane * kBoxBytes, &maps.vc_map, &full_bar[st], lane * 64, m.kh,
+                          m.k_lo + j * kBN);
+          }
+          continue;
+        }
         int32_t blk_next = block_of(0);
         for (int j = 0; j < m.n && ok; ++j) {
           const int pos0 = m.k_lo + j * kBN + page * kPage;
@@ -309,58 +341,80 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
       for (uint32_t i = (c > stages ? c - stages : 0); i < c; ++i) drain_idx(&full_bar[i % stages], i / stages);
     } else if (warp == kMmaWarp) {
       // ---------------------------------------------------------------- MMA issuer
+      // Its path between two MMAs is what the tensor pipe waits for: one branch around each group of
+      // MMAs, descriptors advanced by constants, and waits that pass without further checks.
       const bool leader = tc::elect_one();
+      auto ready = [&](uint64_t* bar, uint32_t index) -> bool {
+        if (mbar_try_wait(bar, index & 1u)) {
+          __syncwarp();
+          return true;
+        }
+        return wait_warp(bar, index);
+      };
+      const uint64_t qdesc = tc::smem_desc(sbase + L::kSmemQ, 16, 1024);
+      const uint64_t kdesc = tc::smem_desc(sbase + L::kSmemK, 16, 1024);
+      const uint64_t vdesc = tc::smem_desc(sbase + L::kSmemV, kBoxBytes, 1024);
       uint32_t qc0 = 0, qc1 = 0, pc0 = 0, pc1 = 0, kvc = 0;
       bool issued = false, ok = true;
       for (uint32_t k = 0; ok && !failed_warp(); ++k) {
         int64_t it;
         if (!(ok = take_item(k, it)) || it < 0) break;
         const Item m = decode_item(a, it, prefix_items);
+        bool copied;
+        if (!(ok = takes_copy(m, copied))) break;
+        const bool pair = kBF16 && !copied;  // P as a hi + lo pair
+        const uint32_t id_pv = kBF16 && copied ? kIdPV16 : kIdPV;
 #pragma unroll 1
         for (int j = 0; j <= m.n && ok; ++j) {
           const uint32_t ki = kvc + j, vi = ki - 1;
-          if (j > 0 && !(ok = wait_warp(&bars.v_full[vi % kVStages], vi / kVStages))) break;
+          if (j > 0 && !(ok = ready(&bars.v_full[vi % kVStages], vi / kVStages))) break;
+          const uint64_t kd = kdesc + (uint64_t)(ki % kKStages) * (L::kTile >> 4);
+          const uint64_t vd = vdesc + (uint64_t)(vi % kVStages) * (L::kTile >> 4);
           bool k_ready = false;
-#pragma unroll 1
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t pc = w ? pc1 : pc0;
-            const int nw = tiles_of(m, w);
-            if (j > 0 && j - 1 < nw) {  // O_w (+)= P_w(j-1) V_(j-1)
-              if (!(ok = wait_warp(&bars.p_full[w], pc))) break;
-              tc::fence_after_sync();
-              const uint32_t pbuf = tmem + w * 128, obuf = tmem + 256 + w * 128;
-              const uint64_t vdesc0 = tc::smem_desc(sbase + L::kSmemV + (vi % kVStages) * L::kTile, kBoxBytes, 1024);
 #pragma unroll
-              for (int kk = 0; kk < kBN / 16; ++kk) {
-                const uint64_t vdesc = vdesc0 + (uint64_t)(kk * (2048 >> 4));
-                const uint32_t pcol = pbuf + (kk >> 1) * 32 + (kk & 1) * 8;
-                if (leader) {
-                  tc::mma_ts(obuf, pcol, vdesc, kIdPV, (j > 1 || kk > 0) ? 1u : 0u);
-                  if (kBF16) tc::mma_ts(obuf, pcol + 16, vdesc, kIdPV, 1u);
+          for (int w = 0; w < 2; ++w) {
+            uint32_t& pc = w ? pc1 : pc0;
+            uint32_t& qc = w ? qc1 : qc0;
+            const int nw = w ? m.n1 : m.n0;
+            if (j > 0 && j - 1 < nw) {  // O_w (+)= P_w(j-1) V_(j-1)
+              if (!(ok = ready(&bars.p_full[w], pc))) break;
+              tc::fence_after_sync();
+              const uint32_t pbuf = tmem + w * 128, obuf = tmem + 256 + w * 128, add = j > 1;
+              if (leader) {
+                if (pair) {
+#pragma unroll
+                  for (int kk = 0; kk < kBN / 16; ++kk) {
+                    const uint32_t pcol = pbuf + (kk >> 1) * 32 + (kk & 1) * 8;
+                    tc::mma_ts(obuf, pcol, vd + (uint64_t)(kk * (2048 >> 4)), kIdPV, kk > 0 ? 1u : add);
+                    tc::mma_ts(obuf, pcol + 16, vd + (uint64_t)(kk * (2048 >> 4)), kIdPV, 1u);
+                  }
+                } else {
+#pragma unroll
+                  for (int kk = 0; kk < kBN / 16; ++kk)
+                    tc::mma_ts(obuf, pbuf + (kk >> 1) * 32 + (kk & 1) * 8, vd + (uint64_t)(kk * (2048 >> 4)), id_pv, kk > 0 ? 1u : add);
                 }
+                if (j == nw) tc::commit(&bars.o_done[w]);
               }
-              if (leader && j == nw) tc::commit(&bars.o_done[w]);
-              if (w) pc1 = pc + 1; else pc0 = pc + 1;
+              __syncwarp();
+              ++pc;
             }
             if (j < nw) {  // S_w(j) = Q_w K_j^T
               if (!k_ready) {
-                if (!(ok = wait_warp(&bars.k_full[ki % kKStages], ki / kKStages))) break;
+                if (!(ok = ready(&bars.k_full[ki % kKStages], ki / kKStages))) break;
                 k_ready = true;
               }
-              if (j == 0 && !(ok = wait_warp(&bars.q_full[w], w ? qc1 : qc0))) break;
-              const uint64_t kdesc0 = tc::smem_desc(sbase + L::kSmemK + (ki % kKStages) * L::kTile, 16, 1024);
-              const uint64_t qdesc0 = tc::smem_desc(sbase + L::kSmemQ + w * L::kTile, 16, 1024);
+              if (j == 0 && !(ok = ready(&bars.q_full[w], qc))) break;
+              if (leader) {
 #pragma unroll
-              for (int kk = 0; kk < D / 16; ++kk) {
-                const uint32_t off = (kk >> 2) * kBoxBytes + (kk & 3) * 32;
-                const uint64_t qdesc = qdesc0 + (uint64_t)(off >> 4), kdesc = kdesc0 + (uint64_t)(off >> 4);
-                if (leader) tc::mma_ss(tmem + w * 128, qdesc, kdesc, kIdQK, kk > 0);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const uint64_t off = (uint64_t)(((kk >> 2) * kBoxBytes + (kk & 3) * 32) >> 4);
+                  tc::mma_ss(tmem + w * 128, qdesc + (uint64_t)(w * (L::kTile >> 4)) + off, kd + off, kIdQK, kk > 0);
+                }
+                tc::commit(&bars.s_full[w]);
+                if (j == nw - 1) tc::commit(&bars.q_empty[w]);
               }
-              if (leader) tc::commit(&bars.s_full[w]);
-              if (j == nw - 1) {
-                if (leader) tc::commit(&bars.q_empty[w]);
-                if (w) ++qc1; else ++qc0;
-              }
+              __syncwarp();
+              if (j == nw - 1) ++qc;
               issued = true;
             }
           }
@@ -379,9 +433,18 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
       // The own kernel needs the plan, not this kernel's results: let it start once the plan is done.
       wait_previous();
       release_dependents();
+      if (a.v_copy) {
+        uint32_t wide = 0;
+        for (int i = lane; i < a.copy_ctas; i += 32) wide |= __ldcg(a.v_wide + i);
+        wide = __any_sync(0xffffffffu, wide != 0);
+        if (lane == 0) {
+          s_copy = !wide;
+          mbar_arrive(&bars.plan);
+        }
+      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax + epilogue
     const int w = warp >> 2, row = tid & (kWg - 1);
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
@@ -400,7 +463,9 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
       // last key the row sees; rows without a token see everything (their results are dropped)
       const int last = m.chunk && row_ok ? m.qpos0 + w * TQ + tl : m.k_end - 1;
       float m_run = -INFINITY, l_run = 0.f;
-      bool ok = true;
+      bool copied;
+      bool ok = takes_copy(m, copied);
+      if (!ok) break;
       for (int j = 0; j < nw; ++j, ++t) {
         if (!(ok = wait_warp(&bars.s_full[w], t))) break;
         tc::fence_after_sync();
@@ -479,38 +544,42 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
         const float kscale = raw ? qk_scale : 1.0f;
         const float2 ks2 = make_float2(kscale, kscale), nmu2 = make_float2(-mu, -mu);
         float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto exp_chunk = [&](const float(&x)[32], int c) {
+        auto exp_chunk = [&](const float(&x)[32], int c, auto as_pair) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 e = tc::fma2(make_float2(x[2 * i], x[2 * i + 1]), ks2, nmu2);
             const float2 pr = i % kPolyEvery == kPolyEvery - 1 ? tc::exp2_poly2(e) : make_float2(tc::ex2(e.x), tc::ex2(e.y));
             ls[i & 1] = tc::add2(ls[i & 1], pr);
-            if constexpr (kBF16) {
+            if constexpr (decltype(as_pair)::value) {
               // hi: the upper 16 bits; lo: the exact rest, rounded
               const uint32_t u0 = __float_as_uint(pr.x), u1 = __float_as_uint(pr.y);
               hi[i] = __byte_perm(u0, u1, 0x7632);
               const float2 r = tc::sub2(pr, make_float2(__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)));
               lo[i] = MMA::pack(r.x, r.y);
             } else {
-              hi[i] = MMA::pack(pr.x, pr.y);
+              hi[i] = mma_op<__half>::pack(pr.x, pr.y);
             }
           }
           tc::st16u(sbuf + c * 32, hi);
-          if constexpr (kBF16) tc::st16u(sbuf + c * 32 + 16, lo);
+          if constexpr (decltype(as_pair)::value) tc::st16u(sbuf + c * 32 + 16, lo);
         };
-        float xa[32], xb[32];
-        tc::ld32(sbuf, xa);
-        tc::wait_ld();
+        auto exp_tile = [&](auto as_pair) {
+          float xa[32], xb[32];
+          tc::ld32(sbuf, xa);
+          tc::wait_ld();
 #pragma unroll 1
-        for (int c = 0; c < kBN / 32; c += 2) {
-          tc::ld32(sbuf + (c + 1) * 32, xb);
-          exp_chunk(xa, c);
-          tc::wait_ld();
-          if (c + 2 < kBN / 32) tc::ld32(sbuf + (c + 2) * 32, xa);
-          exp_chunk(xb, c + 1);
-          tc::wait_ld();
-        }
+          for (int c = 0; c < kBN / 32; c += 2) {
+            tc::ld32(sbuf + (c + 1) * 32, xb);
+            exp_chunk(xa, c, as_pair);
+            tc::wait_ld();
+            if (c + 2 < kBN / 32) tc::ld32(sbuf + (c + 2) * 32, xa);
+            exp_chunk(xb, c + 1, as_pair);
+            tc::wait_ld();
+          }
+        };
+        if (kBF16 && !copied) exp_tile(std::integral_constant<bool, kBF16>());
+        else exp_tile(std::false_type());
         l_run += (ls[0].x + ls[1].x) + (ls[0].y + ls[1].y);
         tc::wait_st();
         tc::fence_before_sync();
@@ -541,15 +610,16 @@ __global__ void __launch_bounds__(kBoundThreads, 1) shared_prefix_tc_kernel(cons
   if (warp == kMmaWarp) tc::dealloc(tmem, 512);
 }
 
-template <typename T, int D>
-cudaError_t launch_tc_t(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms, cudaStream_t stream) {
-  auto kernel = shared_prefix_tc_kernel<T, D>;
+template <typename T, int D, bool BESIDE>
+cudaError_t launch_shape(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms, cudaStream_t stream) {
+  using L = TcLayout<D, BESIDE>;
+  auto kernel = shared_prefix_tc_kernel<T, D, BESIDE>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static std::atomic<uint32_t> ready[64];  // per device: attributes set and checked
   if (!ready[dev & 63].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e != cudaSuccess) return e;
     // both kernels' CTAs share an SM only in the largest shared-memory split
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
@@ -557,10 +627,17 @@ cudaError_t launch_tc_t(const SharedPrefixArgs& a, const SharedPrefixMaps& maps,
     cudaFuncAttributes attr;  // setmaxnreg.inc waits until the launch allocation covers the split
     e = cudaFuncGetAttributes(&attr, kernel);
     if (e != cudaSuccess) return e;
-    if (attr.numRegs * kThreads < kSplitRegs) return cudaErrorInvalidConfiguration;
+    if (attr.numRegs * kThreads < L::kSplitRegs) return cudaErrorInvalidConfiguration;
     ready[dev & 63].store(1, std::memory_order_release);
   }
-  return launch_dependent(kernel, dim3(num_sms), dim3(kThreads), TcLayout<D>::kSmem, stream, a, maps);
+  return launch_dependent(kernel, dim3(num_sms), dim3(kThreads), L::kSmem, stream, a, maps);
+}
+
+template <typename T, int D>
+cudaError_t launch_tc_t(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms, cudaStream_t stream) {
+  if constexpr (D == 128)
+    if (!a.beside) return launch_shape<T, D, false>(a, maps, num_sms, stream);
+  return launch_shape<T, D, true>(a, maps, num_sms, stream);
 }
 
 }  // namespace

@@ -487,6 +487,27 @@ def test_prefix_peaked_scores(new):
     check_prefix(c, scale=1.0)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("value", [None, 60000.0, 70000.0, 1e30, float("inf"), float("nan")])
+def test_prefix_values_beyond_fp16(d, value):
+    """Enough query tiles for the fp16 copy of the prefix's values, with and without a value that does not
+    fit: then the call has to be the one on the bf16 values."""
+    H, KV, B, P = 16, 2, 150, 400
+    c = prefix_case(d, [3] * B, [1] * B, P, H, KV, d)
+    if value is None:
+        check_prefix(c)
+        return
+    c["vc"][c["ptable"][7].long(), 5, 1, 3] = value
+    got, want = prefix_call(c).double().view(B, H, d), prefix64(c).view(B, H, d)
+    touched = torch.zeros(B, H, d, dtype=torch.bool, device="cuda")
+    touched[:, H // 2:, 3] = True  # kv head 1, channel 3
+    close16(prefix_call(c).view(B, H, d)[~touched], want[~touched], 2e-3)
+    if value == value and abs(value) < float("inf"):
+        assert ((got[touched] - want[touched]).abs() <= want[touched].abs() * 2.0 ** -8 + 2e-3).all()
+    else:
+        assert not torch.isfinite(got[touched]).any()
+
+
 def test_prefix_equals_whole_sequences():
     """The same keys as one block table per sequence, through paged_attention."""
     past, new, P, H, KV, d = [40, 7, 0], [1, 1, 1], 320, 32, 8, 128
