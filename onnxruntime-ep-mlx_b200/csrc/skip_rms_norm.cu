@@ -6,8 +6,8 @@
 // Memory bound (about 8 flops per 7 to 8 bytes).  One CTA owns a row and keeps its s in registers
 // (ITEMS vectors of VEC channels per thread), so every input is read once and every output written
 // once; the sum of squares and a row's maximum cross the CTA through shared memory, and a group of
-// channels that lies inside a warp needs shuffles only.  All sums are fp32 and their order is fixed
-// by the row's width, so a row's result does not depend on the batch around it.
+// channels that lies inside a warp needs shuffles only.  With many rows a CTA walks several and has
+// the next row's loads in flight during this row's reductions.  All sums are fp32.
 #include <algorithm>
 
 #include "b200_common.cuh"
@@ -78,151 +78,172 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
-template <typename T, int VEC, int ITEMS, bool FP8>
-__global__ void __launch_bounds__(1024) skip_rms_norm_kernel(const B200SkipRmsNormParams p) {
+// CTAs per SM the walking kernel is built (and launched) for.
+template <int VEC, int ITEMS> constexpr int kWalkers = VEC * ITEMS <= 8 ? 6 : VEC * ITEMS <= 16 ? 4 : 2;
+constexpr int kWalkThreads = 256;
+
+// WALK: rows blockIdx.x, + gridDim.x, ..; at most kWalkThreads threads.  Otherwise row blockIdx.x.
+template <typename T, int VEC, int ITEMS, bool FP8, bool WALK>
+__global__ void __launch_bounds__(WALK ? kWalkThreads : 1024, (WALK ? kWalkers<VEC, ITEMS> : 1))
+    skip_rms_norm_kernel(const __grid_constant__ B200SkipRmsNormParams p) {
   using R = typename Raw<VEC>::type;
-  __shared__ float warp_sum[32];
-  __shared__ int group_max[B200_SKIP_RMS_NORM_MAX_HIDDEN / B200_SKIP_RMS_NORM_MIN_GROUP];
+  // two of each, by the row's parity: a row's values are still read while the next row's are formed
+  __shared__ float warp_sums[2][32];
+  __shared__ int group_maxima[FP8 ? 2 : 1][FP8 ? B200_SKIP_RMS_NORM_MAX_HIDDEN / B200_SKIP_RMS_NORM_MIN_GROUP : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
-  const int64_t row = blockIdx.x;
   const int n = p.hidden / VEC;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_row_stride;
-  const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_row_stride : nullptr;
-  const T* weight = static_cast<const T*>(p.weight);
-
   R xr[ITEMS], rr[ITEMS], wr[ITEMS];
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const int i = tid + k * threads;
-    xr[k] = rr[k] = wr[k] = R{};
-    if (i < n) {
-      xr[k] = *reinterpret_cast<const R*>(x + i * VEC);
-      if (res) rr[k] = *reinterpret_cast<const R*>(res + i * VEC);
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k)
-    if (tid + k * threads < n) wr[k] = __ldg(reinterpret_cast<const R*>(weight) + tid + k * threads);
-
-  float s[ITEMS][VEC], sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    float r[VEC];
-    unpack<T, VEC>(xr[k], s[k]);
-    unpack<T, VEC>(rr[k], r);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      s[k][j] += r[j];
-      sum += s[k][j] * s[k][j];
-    }
-  }
-  if (p.residual_out) {
-    T* ro = static_cast<T*>(p.residual_out) + row * p.residual_out_row_stride;
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-      if (tid + k * threads < n) *reinterpret_cast<R*>(ro + (tid + k * threads) * VEC) = pack<T, VEC>(s[k]);
-  }
-  const int groups = FP8 && p.group_size ? (p.hidden + p.group_size - 1) / p.group_size : 1;
-  if (FP8)
-    for (int i = tid; i < groups; i += threads) group_max[i] = 0;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) warp_sum[warp] = sum;
-  __syncthreads();
-  sum = lane < (threads >> 5) ? warp_sum[lane] : 0.f;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float rstd = 1.0f / sqrtf(sum / (float)p.hidden + p.epsilon);
-
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    float w[VEC];
-    unpack<T, VEC>(wr[k], w);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) s[k][j] = s[k][j] * rstd * w[j];
-  }
-  if constexpr (!FP8) {
-    T* out = static_cast<T*>(p.out) + row * p.out_row_stride;
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-      if (tid + k * threads < n) *reinterpret_cast<R*>(out + (tid + k * threads) * VEC) = pack<T, VEC>(s[k]);
-  } else {
-    uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.out_row_stride;
-    float* scales = p.scales + row * groups;
-    // lanes of one warp that share a group; a group wider than a warp is joined in shared memory
-    const int lanes = p.group_size ? min(32, p.group_size / VEC) : 32;
-    const bool in_warp = p.group_size != 0 && p.group_size <= 32 * VEC;
-    float amax[ITEMS], row_max = 0.f;
+  auto load = [&](int64_t row) {
+    const T* x = static_cast<const T*>(p.x) + row * p.x_row_stride;
+    const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_row_stride : nullptr;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      float m = 0.f;
-      if (tid + k * threads < n) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(s[k][j]));
+      const int i = tid + k * threads;
+      xr[k] = rr[k] = R{};
+      if (i < n) {
+        xr[k] = *reinterpret_cast<const R*>(x + i * VEC);
+        if (res) rr[k] = *reinterpret_cast<const R*>(res + i * VEC);
       }
-      amax[k] = m;
-      row_max = max_nan(row_max, m);
     }
-    if (!p.group_size) {
+  };
+  load(blockIdx.x);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) row_max = max_nan(row_max, __shfl_xor_sync(0xffffffffu, row_max, o));
-      // magnitudes order like their bit patterns, a NaN above all
-      if (lane == 0) atomicMax(&group_max[0], __float_as_int(row_max));
-      __syncthreads();
-      const float scale = max_nan(__int_as_float(group_max[0]), kAmaxFloor) / kFp8Max;
+  for (int k = 0; k < ITEMS; ++k)
+    wr[k] = tid + k * threads < n ? __ldg(reinterpret_cast<const R*>(p.weight) + tid + k * threads) : R{};
+
+  int parity = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1) {
+    float* warp_sum = warp_sums[parity];
+    int* group_max = group_maxima[FP8 ? parity : 0];
+    float s[ITEMS][VEC], sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k) amax[k] = scale;
-      if (tid == 0) scales[0] = scale;
-    } else {
+    for (int k = 0; k < ITEMS; ++k) {
+      float r[VEC];
+      unpack<T, VEC>(xr[k], s[k]);
+      unpack<T, VEC>(rr[k], r);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        s[k][j] += r[j];
+        sum += s[k][j] * s[k][j];
+      }
+    }
+    if (WALK && row + gridDim.x < p.rows) load(row + gridDim.x);
+    if (p.residual_out) {
+      T* ro = static_cast<T*>(p.residual_out) + row * p.residual_out_row_stride;
 #pragma unroll
       for (int k = 0; k < ITEMS; ++k)
-        for (int o = lanes >> 1; o; o >>= 1) amax[k] = max_nan(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], o));
-      if (!in_warp) {
+        if (tid + k * threads < n) *reinterpret_cast<R*>(ro + (tid + k * threads) * VEC) = pack<T, VEC>(s[k]);
+    }
+    const int groups = FP8 && p.group_size ? (p.hidden + p.group_size - 1) / p.group_size : 1;
+    if (FP8)
+      for (int i = tid; i < groups; i += threads) group_max[i] = 0;
 #pragma unroll
-        for (int k = 0; k < ITEMS; ++k)
-          if (lane == 0 && tid + k * threads < n)
-            atomicMax(&group_max[(tid + k * threads) * VEC / p.group_size], __float_as_int(amax[k]));
-        __syncthreads();
-      }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) warp_sum[warp] = sum;
+    __syncthreads();
+    sum = lane < (threads >> 5) ? warp_sum[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float rstd = 1.0f / sqrtf(sum / (float)p.hidden + p.epsilon);
+
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      float w[VEC];
+      unpack<T, VEC>(wr[k], w);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[k][j] = s[k][j] * rstd * w[j];
+    }
+    if constexpr (!FP8) {
+      T* out = static_cast<T*>(p.out) + row * p.out_row_stride;
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        if (tid + k * threads < n) *reinterpret_cast<R*>(out + (tid + k * threads) * VEC) = pack<T, VEC>(s[k]);
+    } else {
+      uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.out_row_stride;
+      float* scales = p.scales + row * groups;
+      // lanes of one warp that share a group; a group wider than a warp is joined in shared memory
+      const int lanes = p.group_size ? min(32, p.group_size / VEC) : 32;
+      const bool in_warp = p.group_size != 0 && p.group_size <= 32 * VEC;
+      float amax[ITEMS], row_max = 0.f;
 #pragma unroll
       for (int k = 0; k < ITEMS; ++k) {
-        const int c = (tid + k * threads) * VEC;
-        if (c >= p.hidden) continue;
-        const int g = c / p.group_size;
-        if (!in_warp) amax[k] = __int_as_float(group_max[g]);
-        amax[k] = max_nan(amax[k], kAmaxFloor) / kFp8Max;
-        if (c % p.group_size == 0) scales[g] = amax[k];
-      }
-    }
+        float m = 0.f;
+        if (tid + k * threads < n) {
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-      if (tid + k * threads < n) store_e4m3<VEC>(out + (tid + k * threads) * VEC, s[k], 1.0f / amax[k]);
+          for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(s[k][j]));
+        }
+        amax[k] = m;
+        row_max = max_nan(row_max, m);
+      }
+      if (!p.group_size) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) row_max = max_nan(row_max, __shfl_xor_sync(0xffffffffu, row_max, o));
+        // magnitudes order like their bit patterns, a NaN above all
+        if (lane == 0) atomicMax(&group_max[0], __float_as_int(row_max));
+        __syncthreads();
+        const float scale = max_nan(__int_as_float(group_max[0]), kAmaxFloor) / kFp8Max;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) amax[k] = scale;
+        if (tid == 0) scales[0] = scale;
+      } else {
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k)
+          for (int o = lanes >> 1; o; o >>= 1) amax[k] = max_nan(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], o));
+        if (!in_warp) {
+#pragma unroll
+          for (int k = 0; k < ITEMS; ++k)
+            if (lane == 0 && tid + k * threads < n)
+              atomicMax(&group_max[(tid + k * threads) * VEC / p.group_size], __float_as_int(amax[k]));
+          __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+          const int c = (tid + k * threads) * VEC;
+          if (c >= p.hidden) continue;
+          const int g = c / p.group_size;
+          if (!in_warp) amax[k] = __int_as_float(group_max[g]);
+          amax[k] = max_nan(amax[k], kAmaxFloor) / kFp8Max;
+          if (c % p.group_size == 0) scales[g] = amax[k];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        if (tid + k * threads < n) store_e4m3<VEC>(out + (tid + k * threads) * VEC, s[k], 1.0f / amax[k]);
+    }
   }
 }
 
-template <typename T, int VEC, int ITEMS>
-void launch_items(const B200SkipRmsNormParams& p, int threads, cudaStream_t stream) {
+template <typename T, int VEC, int ITEMS, bool WALK>
+void launch_items(const B200SkipRmsNormParams& p, int num_sms, cudaStream_t stream) {
+  const int threads = (p.hidden / VEC + 32 * ITEMS - 1) / (32 * ITEMS) * 32;
+  const int grid = WALK ? std::min(p.rows, num_sms * kWalkers<VEC, ITEMS>) : p.rows;
   if (p.out_dtype == B200_DTYPE_FLOAT8E4M3FN)
-    skip_rms_norm_kernel<T, VEC, ITEMS, true><<<p.rows, threads, 0, stream>>>(p);
+    skip_rms_norm_kernel<T, VEC, ITEMS, true, WALK><<<grid, threads, 0, stream>>>(p);
   else
-    skip_rms_norm_kernel<T, VEC, ITEMS, false><<<p.rows, threads, 0, stream>>>(p);
+    skip_rms_norm_kernel<T, VEC, ITEMS, false, WALK><<<grid, threads, 0, stream>>>(p);
 }
 
+// Few rows: as many threads as there are vectors, for the shortest row.  Many rows: at most 256 threads,
+// so several CTAs share an SM and one's reductions overlap another's loads.
 template <typename T, int VEC>
-void launch_vec(const B200SkipRmsNormParams& p, cudaStream_t stream) {
+void launch_vec(const B200SkipRmsNormParams& p, int num_sms, cudaStream_t stream) {
   const int n = p.hidden / VEC;
-  auto threads_for = [&](int items) { return std::min(1024, ((n + items - 1) / items + 31) / 32 * 32); };
-  if (n <= 1024) launch_items<T, VEC, 1>(p, threads_for(1), stream);
-  else if (n <= 2048) launch_items<T, VEC, 2>(p, threads_for(2), stream);
-  else if (n <= 4096) launch_items<T, VEC, 4>(p, threads_for(4), stream);
-  else if constexpr (VEC <= 4) {
-    if (n <= 8192) launch_items<T, VEC, 8>(p, threads_for(8), stream);
-    else if constexpr (VEC == 1) launch_items<T, VEC, 32>(p, threads_for(32), stream);
+  if (p.rows > 4 * num_sms && n <= 4 * kWalkThreads) {
+    if (n <= kWalkThreads) launch_items<T, VEC, 1, true>(p, num_sms, stream);
+    else if (n <= 2 * kWalkThreads) launch_items<T, VEC, 2, true>(p, num_sms, stream);
+    else launch_items<T, VEC, 4, true>(p, num_sms, stream);
+  } else if (n <= 1024) {
+    launch_items<T, VEC, 1, false>(p, num_sms, stream);
+  } else if (n <= 4096) {
+    launch_items<T, VEC, 4, false>(p, num_sms, stream);
+  } else if constexpr (VEC <= 4) {
+    if (n <= 8192) launch_items<T, VEC, 8, false>(p, num_sms, stream);
+    else if constexpr (VEC == 1) launch_items<T, VEC, 32, false>(p, num_sms, stream);
   }
 }
 
 template <typename T>
-void launch_type(const B200SkipRmsNormParams& p, cudaStream_t stream) {
+void launch_type(const B200SkipRmsNormParams& p, int num_sms, cudaStream_t stream) {
   // widest vector that every row of every 16-bit tensor starts on and that divides the row
   const int out16 = p.out_dtype == p.dtype;
   uintptr_t mask = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.residual) |
@@ -232,16 +253,16 @@ void launch_type(const B200SkipRmsNormParams& p, cudaStream_t stream) {
   if (p.residual_out) mask |= (uintptr_t)(p.residual_out_row_stride * 2);
   mask |= out16 ? reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_row_stride * 2)
                 : (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row_stride) * 2;
-  if (mask % 16 == 0) launch_vec<T, 8>(p, stream);
-  else if (mask % 8 == 0) launch_vec<T, 4>(p, stream);
-  else launch_vec<T, 1>(p, stream);
+  if (mask % 16 == 0) launch_vec<T, 8>(p, num_sms, stream);
+  else if (mask % 8 == 0) launch_vec<T, 4>(p, num_sms, stream);
+  else launch_vec<T, 1>(p, num_sms, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_skip_rms_norm(const B200SkipRmsNormParams& p, int, cudaStream_t stream) {
-  if (p.dtype == B200_DTYPE_BFLOAT16) launch_type<__nv_bfloat16>(p, stream);
-  else launch_type<__half>(p, stream);
+cudaError_t launch_skip_rms_norm(const B200SkipRmsNormParams& p, int num_sms, cudaStream_t stream) {
+  if (p.dtype == B200_DTYPE_BFLOAT16) launch_type<__nv_bfloat16>(p, num_sms, stream);
+  else launch_type<__half>(p, num_sms, stream);
   add_launches(1);
   return cudaGetLastError();
 }
