@@ -78,13 +78,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
-// CTAs per SM the walking kernel is built (and launched) for.
-template <int VEC, int ITEMS> constexpr int kWalkers = VEC * ITEMS <= 8 ? 6 : VEC * ITEMS <= 16 ? 4 : 2;
-constexpr int kWalkThreads = 256;
+constexpr int kWalkThreads = 512;  // most threads of a walking CTA; its registers are limited for 1024 per SM
 
 // WALK: rows blockIdx.x, + gridDim.x, ..; at most kWalkThreads threads.  Otherwise row blockIdx.x.
 template <typename T, int VEC, int ITEMS, bool FP8, bool WALK>
-__global__ void __launch_bounds__(WALK ? kWalkThreads : 1024, (WALK ? kWalkers<VEC, ITEMS> : 1))
+__global__ void __launch_bounds__(WALK ? kWalkThreads : 1024, WALK ? 2 : 1)
     skip_rms_norm_kernel(const __grid_constant__ B200SkipRmsNormParams p) {
   using R = typename Raw<VEC>::type;
   // two of each, by the row's parity: a row's values are still read while the next row's are formed
@@ -101,8 +99,8 @@ __global__ void __launch_bounds__(WALK ? kWalkThreads : 1024, (WALK ? kWalkers<V
       const int i = tid + k * threads;
       xr[k] = rr[k] = R{};
       if (i < n) {
-        xr[k] = *reinterpret_cast<const R*>(x + i * VEC);
-        if (res) rr[k] = *reinterpret_cast<const R*>(res + i * VEC);
+        xr[k] = __ldcs(reinterpret_cast<const R*>(x + i * VEC));
+        if (res) rr[k] = __ldcs(reinterpret_cast<const R*>(res + i * VEC));
       }
     }
   };
@@ -161,7 +159,8 @@ __global__ void __launch_bounds__(WALK ? kWalkThreads : 1024, (WALK ? kWalkers<V
     } else {
       uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.out_row_stride;
       float* scales = p.scales + row * groups;
-      // lanes of one warp that share a group; a group wider than a warp is joined in shared memory
+      const int group_log2 = __ffs(p.group_size) - 1;
+    // lanes of one warp that share a group; a group wider than a warp is joined in shared memory
       const int lanes = p.group_size ? min(32, p.group_size / VEC) : 32;
       const bool in_warp = p.group_size != 0 && p.group_size <= 32 * VEC;
       float amax[ITEMS], row_max = 0.f;
@@ -193,17 +192,17 @@ __global__ void __launch_bounds__(WALK ? kWalkThreads : 1024, (WALK ? kWalkers<V
 #pragma unroll
           for (int k = 0; k < ITEMS; ++k)
             if (lane == 0 && tid + k * threads < n)
-              atomicMax(&group_max[(tid + k * threads) * VEC / p.group_size], __float_as_int(amax[k]));
+              atomicMax(&group_max[(tid + k * threads) * VEC >> group_log2], __float_as_int(amax[k]));
           __syncthreads();
         }
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
           const int c = (tid + k * threads) * VEC;
           if (c >= p.hidden) continue;
-          const int g = c / p.group_size;
+          const int g = c >> group_log2;
           if (!in_warp) amax[k] = __int_as_float(group_max[g]);
           amax[k] = max_nan(amax[k], kAmaxFloor) / kFp8Max;
-          if (c % p.group_size == 0) scales[g] = amax[k];
+          if (c == g << group_log2) scales[g] = amax[k];
         }
       }
 #pragma unroll
@@ -216,22 +215,21 @@ __global__ void __launch_bounds__(WALK ? kWalkThreads : 1024, (WALK ? kWalkers<V
 template <typename T, int VEC, int ITEMS, bool WALK>
 void launch_items(const B200SkipRmsNormParams& p, int num_sms, cudaStream_t stream) {
   const int threads = (p.hidden / VEC + 32 * ITEMS - 1) / (32 * ITEMS) * 32;
-  const int grid = WALK ? std::min(p.rows, num_sms * kWalkers<VEC, ITEMS>) : p.rows;
+  const int grid = WALK ? std::min(p.rows, num_sms * std::max(1, 1024 / threads)) : p.rows;
   if (p.out_dtype == B200_DTYPE_FLOAT8E4M3FN)
     skip_rms_norm_kernel<T, VEC, ITEMS, true, WALK><<<grid, threads, 0, stream>>>(p);
   else
     skip_rms_norm_kernel<T, VEC, ITEMS, false, WALK><<<grid, threads, 0, stream>>>(p);
 }
 
-// Few rows: as many threads as there are vectors, for the shortest row.  Many rows: at most 256 threads,
-// so several CTAs share an SM and one's reductions overlap another's loads.
+// Few rows: as many threads as there are vectors, for the shortest row.  Many rows: two vectors per thread
+// in CTAs that walk, 1024 threads per SM (960 and 768 were up to 30 % slower at 8192 channels).
 template <typename T, int VEC>
 void launch_vec(const B200SkipRmsNormParams& p, int num_sms, cudaStream_t stream) {
   const int n = p.hidden / VEC;
-  if (p.rows > 4 * num_sms && n <= 4 * kWalkThreads) {
-    if (n <= kWalkThreads) launch_items<T, VEC, 1, true>(p, num_sms, stream);
-    else if (n <= 2 * kWalkThreads) launch_items<T, VEC, 2, true>(p, num_sms, stream);
-    else launch_items<T, VEC, 4, true>(p, num_sms, stream);
+  if (p.rows > 4 * num_sms && n <= 2 * kWalkThreads) {
+    if (n <= 128) launch_items<T, VEC, 1, true>(p, num_sms, stream);
+    else launch_items<T, VEC, 2, true>(p, num_sms, stream);
   } else if (n <= 1024) {
     launch_items<T, VEC, 1, false>(p, num_sms, stream);
   } else if (n <= 4096) {
