@@ -11,11 +11,12 @@
 //
 // A query tile is 128 rows = tile_tokens tokens x g heads.  Roles, joined by mbarriers only:
 //   warps 0-3 / 4-7  softmax and epilogue of query tile 0 / 1, one row per thread = tensor-memory lane
-//   warp 8           takes items, loads Q and K tiles by TMA (8 pages of 16 slots per 128-key tile)
+//   warp 8           loads Q and K tiles by TMA (8 pages of 16 slots per 128-key tile)
 //   warp 9           issues the MMAs: per K/V tile j PV0(j-1), S0(j), PV1(j-1), S1(j), so the tensor
 //                    pipe works on one query tile while the other one's softmax runs
 //   warp 10          loads V tiles
-//   warp 11          lets the own kernel start when the plan is done
+//   warp 11          takes items and works out what they are, up to two ahead of the others; lets the
+//                    own kernel start when the plan is done
 // S = Q K^T (both operands in shared memory), O += P V with P in tensor memory over S's columns and V as
 // the MN-major operand in the cache's [key][channel] order.  P is one fp16 value per key against fp16
 // values (fp16 calls, or bf16 calls on the plan's fp16 copy of the prefix's values) and a hi + lo pair
@@ -39,7 +40,9 @@ constexpr int kBN = kPrefixKeys;    // keys per tile
 constexpr int kPage = 16;           // slots per TMA box
 constexpr int kBoxBytes = 128 * 128;  // [128 rows][64 channels]
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kPolyEvery = 4;       // every 4th exponential pair on the FMA pipe
+constexpr int kPolyEvery = 8;       // every 4th exponential pair on the FMA pipe
+// Head size 64: O takes half of its 128 columns, single P the other half (columns from S to P).
+constexpr uint32_t kPBeside = 256 + 64;
 
 // Two shapes of the kernel.  BESIDE: 160 KB of shared memory and 128 registers per thread at launch (its
 // launch bound of 512 threads sets that), so a CTA of the own kernel fits on the SM beside it; for head
@@ -49,10 +52,11 @@ template <int D, bool BESIDE>
 struct TcLayout {
   static constexpr int kBoxes = D / 64;
   static constexpr int kTile = kBoxes * kBoxBytes;
-  static constexpr int kKStages = D == 64 ? 4 : BESIDE ? 1 : 2;
-  static constexpr int kVStages = D == 64 ? 4 : BESIDE ? 2 : 3;
+  static constexpr int kQBuffers = D == 64 ? 2 : 1;  // per query tile
+  static constexpr int kKStages = D == 64 ? 3 : BESIDE ? 1 : 2;
+  static constexpr int kVStages = D == 64 ? 3 : BESIDE ? 2 : 3;
   static constexpr int kSmemQ = 0;
-  static constexpr int kSmemK = 2 * kTile;
+  static constexpr int kSmemK = 2 * kQBuffers * kTile;
   static constexpr int kSmemV = kSmemK + kKStages * kTile;
   static constexpr int kSmem = kSmemV + kVStages * kTile;
   // setmaxnreg split of the registers per thread at launch
@@ -65,19 +69,48 @@ struct TcLayout {
 
 constexpr int kWg = 128;
 constexpr int kThreads = 3 * kWg;
-constexpr int kLoadWarp = 8, kMmaWarp = 9, kVLoadWarp = 10;
-constexpr int kSched = 4;  // slots of the item queue
-constexpr int kTakers = 2 * kWg / 32 + 2;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kVLoadWarp = 10;  // warp 11: scheduler
+constexpr int kSched = 2;  // slots of the item queue
+constexpr int kTakers = 2 * kWg / 32 + 3;  // softmax, load, MMA and V load warps
+
+// The whole warp waits for a phase, at most kWaitLimitNs, and not once another role has given up.  The
+// roles' code together has to stay in the SM's instruction cache (a role that runs code the others
+// have evicted pays hundreds of cycles a line), so the loop stays rolled and is a call where a role has
+// the registers for one.
+__device__ __forceinline__ bool wait_inline(uint64_t* bar, uint32_t parity, volatile int* failed, int* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t start = globaltimer_ns();
+#pragma unroll 1
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if (__any_sync(0xffffffffu, globaltimer_ns() - start > kWaitLimitNs || *failed != 0)) {
+      if (*failed == 0) set_status(status, kStatusTimeout);
+      *failed = 1;
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __noinline__ bool wait_call(uint64_t* bar, uint32_t parity, volatile int* failed, int* status) {
+  return wait_inline(bar, parity, failed, status);
+}
+// After a failure, too: a bounded wait for a copy or commit this CTA issued.
+__device__ __forceinline__ void wait_drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t start = globaltimer_ns();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - start > kWaitLimitNs) return;
+}
 
 struct Bars {
-  uint64_t q_full[2], q_empty[2];
-  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t q_full[2][2], q_empty[2][2];
+  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
+  uint64_t s_full[2], p_full[2], o_done[2], pv_done[2];
   uint64_t drain, plan;
   uint64_t sched_full[kSched], sched_empty[kSched];
 };
 
 struct Item {
+  int stop;                      // no more items
   int chunk, kh, tok0, tok_end;  // tokens [tok0, tok_end) are the sequence's (prefix: the batch's) from the first tile on
   int qpos0;                     // chunk: own position of token tok0
   int k_lo, k_valid;             // first key; keys of the table that hold data
@@ -87,7 +120,8 @@ struct Item {
   int64_t slab;
 };
 
-__device__ __forceinline__ Item decode_item(const SharedPrefixArgs& a, int64_t it, int64_t prefix_items) {
+// The whole warp.
+__device__ __forceinline__ Item decode_item(const SharedPrefixArgs& a, int64_t it, int64_t prefix_items, int lane) {
   Item m{};
   const int KV = a.p.kv_num_heads, TQ = a.tile_tokens;
   if (it < prefix_items) {  // ((range, kv head), pair): neighbours share their K/V tiles in L2
@@ -111,10 +145,12 @@ __device__ __forceinline__ Item decode_item(const SharedPrefixArgs& a, int64_t i
   const int64_t pair_global = pairs - 1 - it / KV;  // later tiles, which see more keys, first
   m.chunk = 1;
   m.kh = (int)(it % KV);
-  int lo = 0, hi = a.p.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldcg(a.seq_pairs + mid) <= pair_global) lo = mid; else hi = mid - 1;
+  int lo = 0, hi = a.p.batch;  // the largest lo with seq_pairs[lo] <= pair_global, 32 candidates at a time
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const unsigned le = __ballot_sync(0xffffffffu, at < hi && __ldcg(a.seq_pairs + min(at, a.p.batch)) <= pair_global);
+    lo += (__popc(le) - 1) * step;
+    hi = min(hi, lo + step);
   }
   const int q0 = (int)(pair_global - __ldcg(a.seq_pairs + lo)) * 2 * TQ;
   const int c0 = a.p.cumulative_sequence_length[lo], c1 = a.p.cumulative_sequence_length[lo + 1];
@@ -169,7 +205,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
   __shared__ __align__(8) Bars bars;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int s_failed, s_copy;  // s_copy: prefix items take the values' fp16 copy
-  __shared__ volatile long long s_item[kSched];
+  __shared__ Item s_items[kSched];
 
   const B200SharedPrefixParams& p = a.p;
   const uint32_t sbase = smem_u32(smem);
@@ -179,13 +215,16 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
   if (warp == kMmaWarp) tc::alloc(&tmem_slot, 512);
   if (tid == 0) {
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&bars.q_full[w], 1);
-      mbar_init(&bars.q_empty[w], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars.q_full[w][i], 1);
+        mbar_init(&bars.q_empty[w][i], 1);
+      }
       mbar_init(&bars.s_full[w], 1);
       mbar_init(&bars.p_full[w], kWg);
       mbar_init(&bars.o_done[w], 1);
+      mbar_init(&bars.pv_done[w], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&bars.k_full[i], 1);
       mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_full[i], 1);
@@ -204,54 +243,32 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const int64_t prefix_items = (int64_t)a.splits * p.kv_num_heads * a.query_pairs;
 
-  auto wait_idx = [&](uint64_t* bar, uint32_t index) -> bool {  // completion `index` of a barrier
-    if (s_failed) return false;
-    if (mbar_wait(bar, index & 1u)) return true;
-    set_status(p.device_status, kStatusTimeout);
-    s_failed = 1;
-    return false;
+  // Completion `index` of a barrier, for the whole warp.
+  auto wait_softmax = [&](uint64_t* bar, uint32_t index) -> bool {
+    return wait_inline(bar, index & 1u, &s_failed, p.device_status);
   };
-  auto wait_warp = [&](uint64_t* bar, uint32_t index) -> bool { return __all_sync(0xffffffffu, wait_idx(bar, index)); };
+  auto wait_warp = [&](uint64_t* bar, uint32_t index) -> bool {  // control warps
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, index & 1u)) || wait_call(bar, index & 1u, &s_failed, p.device_status);
+  };
   auto failed_warp = [&]() -> bool { return __any_sync(0xffffffffu, s_failed != 0); };
-  auto drain_idx = [&](uint64_t* bar, uint32_t index) { mbar_wait(bar, index & 1u); };
-  // Warp 8 hands out the CTA's k-th item (-1: no more).  The first is the CTA's own and, if it lies in
-  // the prefix, needs nothing of the plan, which may still be running then.
-  auto fetch_item = [&](uint32_t k, int64_t& it) -> bool {
+  auto drain_idx = [&](uint64_t* bar, uint32_t index) { wait_drain(bar, index & 1u); };
+  // The CTA's k-th item, from warp 11.
+  auto take_item = [&](uint32_t k, Item& m, auto wait) -> bool {
     const uint32_t slot = k % kSched;
-    if (k >= (uint32_t)kSched && !wait_warp(&bars.sched_empty[slot], k / kSched - 1)) return false;
-    long long v = blockIdx.x;
-    if (k > 0 || v >= prefix_items) {
-      wait_previous();
-      if (lane == 0) {
-        if (k > 0) v = (long long)gridDim.x + (long long)atomicAdd(a.next_item, 1ull);
-        if (v >= prefix_items + (long long)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads) v = -1;
-      }
-    }
-    if (lane == 0) {
-      s_item[slot] = v;
-      mbar_arrive(&bars.sched_full[slot]);
-    }
-    it = __shfl_sync(0xffffffffu, v, 0);
-    return true;
-  };
-  auto take_item = [&](uint32_t k, int64_t& it) -> bool {
-    const uint32_t slot = k % kSched;
-    if (!wait_warp(&bars.sched_full[slot], k / kSched)) return false;
-    it = s_item[slot];
+    if (!wait(&bars.sched_full[slot], k / kSched)) return false;
+    m = s_items[slot];
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars.sched_empty[slot]);
-    return true;
+    return !m.stop;
   };
-
   // Whether an item's values come from the fp16 copy; waits for the plan (which decides it) at the first
   // prefix item of a call that made the copy.
   bool plan_seen = false;
-  auto takes_copy = [&](const Item& m, bool& copy) -> bool {
+  auto takes_copy = [&](const Item& m, bool& copy, auto wait) -> bool {
     copy = false;
     if (!a.v_copy || m.chunk) return true;
-    if (!plan_seen && !wait_warp(&bars.plan, 0)) return false;
+    if (!plan_seen && !wait(&bars.plan, 0)) return false;
     plan_seen = true;
     copy = s_copy != 0;
     return true;
@@ -274,21 +291,21 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
       const bool loader = lane < 8 * L::kBoxes;
       bool ok = true;
       for (uint32_t k = 0; ok && !failed_warp(); ++k) {
-        int64_t it;
-        if (!(ok = is_v ? take_item(k, it) : fetch_item(k, it)) || it < 0) break;
-        const Item m = decode_item(a, it, prefix_items);
+        Item m;
+        if (!take_item(k, m, wait_warp)) break;
         bool copied = false;
-        if (is_v && !(ok = takes_copy(m, copied))) break;
+        if (is_v && !(ok = takes_copy(m, copied, wait_warp))) break;
         if (!is_v) {
           for (int w = 0; w < 2 && ok; ++w) {
             if (tiles_of(m, w) == 0) continue;
             const uint32_t qc = w ? qc1 : qc0;
-            if (qc > 0 && !(ok = wait_warp(&bars.q_empty[w], qc - 1))) break;
-            if (lane == 0) mbar_arrive_expect_tx(&bars.q_full[w], q_bytes);
+            const uint32_t qb = qc % L::kQBuffers, use = qc / L::kQBuffers;
+            if (use > 0 && !(ok = wait_warp(&bars.q_empty[w][qb], use - 1))) break;
+            if (lane == 0) mbar_arrive_expect_tx(&bars.q_full[w][qb], q_bytes);
             __syncwarp();
             if (lane < L::kBoxes)
-              tma_load_3d(smem + L::kSmemQ + w * L::kTile + lane * kBoxBytes, &maps.q_map, &bars.q_full[w], lane * 64,
-                          m.kh * g, m.tok0 + w * TQ);
+              tma_load_3d(smem + L::kSmemQ + (w * L::kQBuffers + qb) * L::kTile + lane * kBoxBytes, &maps.q_map,
+                          &bars.q_full[w][qb], lane * 64, m.kh * g, m.tok0 + w * TQ);
             if (w) qc1 = qc + 1; else qc0 = qc + 1;
           }
         }
@@ -336,52 +353,47 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
           ++c;
         }
       }
-      if (qc0 > 0) drain_idx(&bars.q_full[0], qc0 - 1);
-      if (qc1 > 0) drain_idx(&bars.q_full[1], qc1 - 1);
+      for (uint32_t w = 0; w < 2; ++w) {
+        const uint32_t qc = w ? qc1 : qc0;
+        for (uint32_t i = (qc > L::kQBuffers ? qc - L::kQBuffers : 0); i < qc; ++i)
+          drain_idx(&bars.q_full[w][i % L::kQBuffers], i / L::kQBuffers);
+      }
       for (uint32_t i = (c > stages ? c - stages : 0); i < c; ++i) drain_idx(&full_bar[i % stages], i / stages);
     } else if (warp == kMmaWarp) {
       // ---------------------------------------------------------------- MMA issuer
       // Its path between two MMAs is what the tensor pipe waits for: one branch around each group of
-      // MMAs, descriptors advanced by constants, and waits that pass without further checks.
+      // MMAs, descriptors advanced by constants.
       const bool leader = tc::elect_one();
-      auto ready = [&](uint64_t* bar, uint32_t index) -> bool {
-        if (mbar_try_wait(bar, index & 1u)) {
-          __syncwarp();
-          return true;
-        }
-        return wait_warp(bar, index);
-      };
       const uint64_t qdesc = tc::smem_desc(sbase + L::kSmemQ, 16, 1024);
       const uint64_t kdesc = tc::smem_desc(sbase + L::kSmemK, 16, 1024);
       const uint64_t vdesc = tc::smem_desc(sbase + L::kSmemV, kBoxBytes, 1024);
       uint32_t qc0 = 0, qc1 = 0, pc0 = 0, pc1 = 0, kvc = 0;
       bool issued = false, ok = true;
       for (uint32_t k = 0; ok && !failed_warp(); ++k) {
-        int64_t it;
-        if (!(ok = take_item(k, it)) || it < 0) break;
-        const Item m = decode_item(a, it, prefix_items);
+        Item m;
+        if (!take_item(k, m, wait_warp)) break;
         bool copied;
-        if (!(ok = takes_copy(m, copied))) break;
+        if (!(ok = takes_copy(m, copied, wait_warp))) break;
         const bool pair = kBF16 && !copied;  // P as a hi + lo pair
         const uint32_t id_pv = kBF16 && copied ? kIdPV16 : kIdPV;
 #pragma unroll 1
         for (int j = 0; j <= m.n && ok; ++j) {
           const uint32_t ki = kvc + j, vi = ki - 1;
-          if (j > 0 && !(ok = ready(&bars.v_full[vi % kVStages], vi / kVStages))) break;
           const uint64_t kd = kdesc + (uint64_t)(ki % kKStages) * (L::kTile >> 4);
           const uint64_t vd = vdesc + (uint64_t)(vi % kVStages) * (L::kTile >> 4);
-          bool k_ready = false;
-#pragma unroll
+          bool k_ready = false, v_ready = false;
+#pragma unroll 1
           for (int w = 0; w < 2; ++w) {
-            uint32_t& pc = w ? pc1 : pc0;
-            uint32_t& qc = w ? qc1 : qc0;
+            const uint32_t pc = w ? pc1 : pc0, qc = w ? qc1 : qc0;
             const int nw = w ? m.n1 : m.n0;
-            if (j > 0 && j - 1 < nw) {  // O_w (+)= P_w(j-1) V_(j-1)
-              if (!(ok = ready(&bars.p_full[w], pc))) break;
-              tc::fence_after_sync();
-              const uint32_t pbuf = tmem + w * 128, obuf = tmem + 256 + w * 128, add = j > 1;
+            const bool has_pv = j > 0 && j - 1 < nw, has_s = j < nw;
+            auto issue_pv = [&]() -> bool {  // O_w (+)= P_w(j-1) V_(j-1)
+              if (!v_ready && !wait_warp(&bars.v_full[vi % kVStages], vi / kVStages)) return false;
+              v_ready = true;
+              const uint32_t obuf = tmem + 256 + w * 128, add = j > 1;
               if (leader) {
                 if (pair) {
+                  const uint32_t pbuf = tmem + w * 128;
 #pragma unroll
                   for (int kk = 0; kk < kBN / 16; ++kk) {
                     const uint32_t pcol = pbuf + (kk >> 1) * 32 + (kk & 1) * 8;
@@ -389,33 +401,50 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
                     tc::mma_ts(obuf, pcol + 16, vd + (uint64_t)(kk * (2048 >> 4)), kIdPV, 1u);
                   }
                 } else {
+                  const uint32_t pbuf = tmem + (D == 64 ? kPBeside : 0) + w * 128;
 #pragma unroll
                   for (int kk = 0; kk < kBN / 16; ++kk)
-                    tc::mma_ts(obuf, pbuf + (kk >> 1) * 32 + (kk & 1) * 8, vd + (uint64_t)(kk * (2048 >> 4)), id_pv, kk > 0 ? 1u : add);
+                    tc::mma_ts(obuf, pbuf + (D == 64 ? kk * 8 : (kk >> 1) * 32 + (kk & 1) * 8), vd + (uint64_t)(kk * (2048 >> 4)),
+                               id_pv, kk > 0 ? 1u : add);
                 }
+                tc::commit(&bars.pv_done[w]);
                 if (j == nw) tc::commit(&bars.o_done[w]);
               }
               __syncwarp();
-              ++pc;
-            }
-            if (j < nw) {  // S_w(j) = Q_w K_j^T
-              if (!k_ready) {
-                if (!(ok = ready(&bars.k_full[ki % kKStages], ki / kKStages))) break;
-                k_ready = true;
-              }
-              if (j == 0 && !(ok = ready(&bars.q_full[w], qc))) break;
+              if (w) ++pc1; else ++pc0;
+              return true;
+            };
+            auto issue_s = [&]() -> bool {  // S_w(j) = Q_w K_j^T
+              if (!k_ready && !wait_warp(&bars.k_full[ki % kKStages], ki / kKStages)) return false;
+              k_ready = true;
+              const uint32_t qb = qc % L::kQBuffers;
+              if (j == 0 && !wait_warp(&bars.q_full[w][qb], qc / L::kQBuffers)) return false;
               if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                   const uint64_t off = (uint64_t)(((kk >> 2) * kBoxBytes + (kk & 3) * 32) >> 4);
-                  tc::mma_ss(tmem + w * 128, qdesc + (uint64_t)(w * (L::kTile >> 4)) + off, kd + off, kIdQK, kk > 0);
+                  tc::mma_ss(tmem + w * 128, qdesc + (uint64_t)((w * L::kQBuffers + qb) * (L::kTile >> 4)) + off, kd + off, kIdQK, kk > 0);
                 }
                 tc::commit(&bars.s_full[w]);
-                if (j == nw - 1) tc::commit(&bars.q_empty[w]);
+                if (j == nw - 1) tc::commit(&bars.q_empty[w][qb]);
               }
               __syncwarp();
-              if (j == nw - 1) ++qc;
+              if (j == nw - 1) {
+                if (w) ++qc1; else ++qc0;
+              }
               issued = true;
+              return true;
+            };
+            if (has_pv) {
+              if (!(ok = wait_warp(&bars.p_full[w], pc))) break;
+              tc::fence_after_sync();
+            }
+            if (D == 64 && !pair) {  // P lies beside S: the next scores do not wait for P V
+              if (has_s && !(ok = issue_s())) break;
+              if (has_pv && !(ok = issue_pv())) break;
+            } else {
+              if (has_pv && !(ok = issue_pv())) break;
+              if (has_s && !(ok = issue_s())) break;
             }
           }
           if (!ok) break;
@@ -430,17 +459,47 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
       }
       __syncwarp();
     } else {
-      // The own kernel needs the plan, not this kernel's results: let it start once the plan is done.
-      wait_previous();
-      release_dependents();
-      if (a.v_copy) {
-        uint32_t wide = 0;
-        for (int i = lane; i < a.copy_ctas; i += 32) wide |= __ldcg(a.v_wide + i);
-        wide = __any_sync(0xffffffffu, wide != 0);
-        if (lane == 0) {
-          s_copy = !wide;
-          mbar_arrive(&bars.plan);
+      // ---------------------------------------------------------------- scheduler
+      // The first item is the CTA's own and, if it lies in the prefix, needs nothing of the plan, which
+      // may still be running then.
+      const int64_t prefix_items = (int64_t)a.splits * p.kv_num_heads * a.query_pairs;
+      bool planned = false;
+      int64_t items = 0;
+      for (uint32_t k = 0; !failed_warp(); ++k) {
+        const uint32_t slot = k % kSched;
+        if (k >= (uint32_t)kSched && !wait_warp(&bars.sched_empty[slot], k / kSched - 1)) break;
+        int64_t it = blockIdx.x;
+        if (!planned && (k > 0 || it >= prefix_items)) {
+          planned = true;
+          // The own kernel needs the plan, not this kernel's results: let it start once the plan is done.
+          wait_previous();
+          release_dependents();
+          items = prefix_items + (int64_t)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads;
+          if (a.v_copy) {
+            uint32_t wide = 0;
+            for (int i = lane; i < a.copy_ctas; i += 32) wide |= __ldcg(a.v_wide + i);
+            wide = __any_sync(0xffffffffu, wide != 0);
+            if (lane == 0) {
+              s_copy = !wide;
+              mbar_arrive(&bars.plan);
+            }
+          }
         }
+        if (k > 0) {
+          unsigned long long next = 0;
+          if (lane == 0) next = atomicAdd(a.next_item, 1ull);
+          it = gridDim.x + (int64_t)__shfl_sync(0xffffffffu, next, 0);
+        }
+        const bool stop = planned && it >= items;
+        Item m{};
+        if (!stop) m = decode_item(a, it, prefix_items, lane);
+        m.stop = stop;
+        if (lane == 0) {
+          s_items[slot] = m;
+          mbar_arrive(&bars.sched_full[slot]);
+        }
+        __syncwarp();
+        if (stop) break;
       }
     }
   } else {
@@ -453,9 +512,8 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
     const int tl = row / g, hl = row % g;
     uint32_t t = 0, items = 0;
     for (uint32_t k = 0; !failed_warp(); ++k) {
-      int64_t it;
-      if (!take_item(k, it) || it < 0) break;
-      const Item m = decode_item(a, it, prefix_items);
+      Item m;
+      if (!take_item(k, m, wait_softmax)) break;
       const int nw = tiles_of(m, w);
       if (nw == 0) continue;
       const int tok = m.tok0 + w * TQ + tl;
@@ -464,129 +522,164 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
       const int last = m.chunk && row_ok ? m.qpos0 + w * TQ + tl : m.k_end - 1;
       float m_run = -INFINITY, l_run = 0.f;
       bool copied;
-      bool ok = takes_copy(m, copied);
+      bool ok = takes_copy(m, copied, wait_softmax);
       if (!ok) break;
       for (int j = 0; j < nw; ++j, ++t) {
-        if (!(ok = wait_warp(&bars.s_full[w], t))) break;
+        if (!(ok = wait_softmax(&bars.s_full[w], t))) break;
         tc::fence_after_sync();
         const int kbase = m.k_lo + j * kBN;
         // Unmasked tiles keep raw scores, the scale goes into the exponent's FMA; others are rewritten
         // in place as scaled log2 values.  Warp-uniform.
         const bool raw = __all_sync(0xffffffffu, kbase + kBN - 1 <= last) && p.softcap <= 0.f && qk_scale > 0.f;
-        float mx[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mx[r] = -INFINITY;
-        if (raw) {
-#pragma unroll
-          for (int c = 0; c < kBN / 32; c += 2) {
-            float xa[32], xb[32];
-            tc::ld32(sbuf + c * 32, xa);
-            tc::ld32(sbuf + (c + 1) * 32, xb);
-            tc::wait_ld();
+        // P per 32-column chunk: bf16 pairs over the chunk's S (hi halves, then lo halves), single fp16
+        // values over the chunk's first 16 columns or, for head size 64, beside S where O leaves room.
+        const bool single = !kBF16 || copied;
+        const uint32_t pbuf = D == 64 && single ? sbuf + kPBeside : sbuf;
+        const int pstep = D == 64 && single ? 16 : 32;
+        bool pv_waited = j == 0 || !(D == 64 && single);  // else S of this tile says that P V of the last is done
+        auto wait_pv = [&]() -> bool {
+          if (pv_waited) return true;
+          pv_waited = true;
+          if (!wait_softmax(&bars.pv_done[w], t - 1)) return false;
+          tc::fence_after_sync();
+          return true;
+        };
+        float2 ls[2];
+        // P = 2^(x * scale - m_run) over the tile, every kPolyEvery-th pair on the FMA pipe; returns the
+        // largest x * scale.  Each chunk of S is read before P may overwrite it.
+        auto exponentials = [&](float scale, auto as_pair) -> float {
+          const float mu = m_run == -INFINITY ? 0.f : m_run;
+          const float2 ks2 = make_float2(scale, scale), nmu2 = make_float2(-mu, -mu);
+          float mx[2] = {-INFINITY, -INFINITY};
+          ls[0] = ls[1] = make_float2(0.f, 0.f);
+          auto chunk = [&](const float(&x)[32], int c) {
+            uint32_t hi[16], lo[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              mx[i & 3] = tc::max3(mx[i & 3], xa[2 * i], xa[2 * i + 1]);
-              mx[i & 3] = tc::max3(mx[i & 3], xb[2 * i], xb[2 * i + 1]);
-            }
-          }
-        } else {
-          const int vhi = last - kbase;
-#pragma unroll 1
-          for (int c = 0; c < kBN / 32; ++c) {
-            float x[32];
-            tc::ld32(sbuf + c * 32, x);
-            tc::wait_ld();
-            if (p.softcap > 0.f) {
-              // cap tanh(y / cap), tanh(u) = 1 - 2 / (1 + e^(2u))
-              const float two_log2e_over_cap = 2.f * kLog2e / p.softcap, cap_log2e = p.softcap * kLog2e;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float e = tc::ex2(fminf(x[i] * qk_scale * two_log2e_over_cap, 126.f));
-                x[i] = cap_log2e * (1.f - __fdividef(2.f, 1.f + e));
+              if (D == 64 && !decltype(as_pair)::value) mx[i & 1] = tc::max3(mx[i & 1], x[2 * i], x[2 * i + 1]);
+              const float2 e = tc::fma2(make_float2(x[2 * i], x[2 * i + 1]), ks2, nmu2);
+              const float2 pr = kPolyEvery > 0 && i % (kPolyEvery > 0 ? kPolyEvery : 1) == kPolyEvery - 1 ? tc::exp2_poly2(e) : make_float2(tc::ex2(e.x), tc::ex2(e.y));
+              ls[i & 1] = tc::add2(ls[i & 1], pr);
+              if constexpr (decltype(as_pair)::value) {
+                // hi: the upper 16 bits; lo: the exact rest, rounded
+                const uint32_t u0 = __float_as_uint(pr.x), u1 = __float_as_uint(pr.y);
+                hi[i] = __byte_perm(u0, u1, 0x7632);
+                const float2 r = tc::sub2(pr, make_float2(__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)));
+                lo[i] = MMA::pack(r.x, r.y);
+              } else {
+                hi[i] = mma_op<__half>::pack(pr.x, pr.y);
               }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] *= qk_scale;
             }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = c * 32 + i <= vhi ? x[i] : -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx[i & 3] = tc::max3(mx[i & 3], x[2 * i], x[2 * i + 1]);
-            tc::st32(sbuf + c * 32, x);
-          }
-          tc::wait_st();
-        }
-        float m_tile = tc::max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
-        if (raw) m_tile *= qk_scale;
-        const float m_new = fmaxf(m_run, m_tile);
-        const bool grow = m_new > m_run + 8.0f;
-        const float alpha = (grow && m_run != -INFINITY) ? tc::ex2(m_run - m_new) : 1.0f;
-        if (grow) {
-          l_run *= (m_run == -INFINITY ? 0.f : alpha);
-          m_run = m_new;
-        }
-        if (j > 0 && __any_sync(0xffffffffu, grow && alpha != 1.0f)) {
-          // s_full of tile j also says that P V of tile j - 1 has landed in O
-#pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            float r[16];
-            tc::ld16(obuf + c * 16, r);
-            tc::wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] *= alpha;
-            tc::st16(obuf + c * 16, r);
-          }
-          tc::wait_st();
-        }
-        // P = 2^(x - mu) per 32-column chunk over the chunk's first 16 columns (bf16: lo halves over
-        // the last 16); each chunk is read before it is overwritten
-        const float mu = m_run == -INFINITY ? 0.f : m_run;
-        const float kscale = raw ? qk_scale : 1.0f;
-        const float2 ks2 = make_float2(kscale, kscale), nmu2 = make_float2(-mu, -mu);
-        float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto exp_chunk = [&](const float(&x)[32], int c, auto as_pair) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 e = tc::fma2(make_float2(x[2 * i], x[2 * i + 1]), ks2, nmu2);
-            const float2 pr = i % kPolyEvery == kPolyEvery - 1 ? tc::exp2_poly2(e) : make_float2(tc::ex2(e.x), tc::ex2(e.y));
-            ls[i & 1] = tc::add2(ls[i & 1], pr);
-            if constexpr (decltype(as_pair)::value) {
-              // hi: the upper 16 bits; lo: the exact rest, rounded
-              const uint32_t u0 = __float_as_uint(pr.x), u1 = __float_as_uint(pr.y);
-              hi[i] = __byte_perm(u0, u1, 0x7632);
-              const float2 r = tc::sub2(pr, make_float2(__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)));
-              lo[i] = MMA::pack(r.x, r.y);
-            } else {
-              hi[i] = mma_op<__half>::pack(pr.x, pr.y);
-            }
-          }
-          tc::st16u(sbuf + c * 32, hi);
-          if constexpr (decltype(as_pair)::value) tc::st16u(sbuf + c * 32 + 16, lo);
-        };
-        auto exp_tile = [&](auto as_pair) {
+            tc::st16u(pbuf + c * pstep, hi);
+            if constexpr (decltype(as_pair)::value) tc::st16u(pbuf + c * 32 + 16, lo);
+          };
           float xa[32], xb[32];
           tc::ld32(sbuf, xa);
           tc::wait_ld();
+          ok = wait_pv();
 #pragma unroll 1
           for (int c = 0; c < kBN / 32; c += 2) {
             tc::ld32(sbuf + (c + 1) * 32, xb);
-            exp_chunk(xa, c, as_pair);
+            chunk(xa, c);
             tc::wait_ld();
             if (c + 2 < kBN / 32) tc::ld32(sbuf + (c + 2) * 32, xa);
-            exp_chunk(xb, c + 1, as_pair);
+            chunk(xb, c + 1);
             tc::wait_ld();
           }
+          return fmaxf(mx[0], mx[1]) * scale;
         };
-        if (kBF16 && !copied) exp_tile(std::integral_constant<bool, kBF16>());
-        else exp_tile(std::false_type());
+        // The running maximum takes in `m_tile`, and O and l follow, where it grows by more than 2^8.
+        auto raise_maximum = [&](float m_tile) {
+          const float m_new = fmaxf(m_run, m_tile);
+          const bool grow = m_new > m_run + 8.0f;
+          const float alpha = (grow && m_run != -INFINITY) ? tc::ex2(m_run - m_new) : 1.0f;
+          if (grow) {
+            l_run *= (m_run == -INFINITY ? 0.f : alpha);
+            m_run = m_new;
+          }
+          if (j > 0 && __any_sync(0xffffffffu, grow && alpha != 1.0f)) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              float r[16];
+              tc::ld16(obuf + c * 16, r);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) r[i] *= alpha;
+              tc::st16(obuf + c * 16, r);
+            }
+            tc::wait_st();
+          }
+        };
+        // Where P does not overwrite S, a tile takes one pass with the maximum as it stands: right unless
+        // a score exceeds it by more than 2^8, which the pass finds out, and then a second one follows.
+        const bool one_pass = D == 64 && single && raw && __all_sync(0xffffffffu, m_run != -INFINITY);
+        if (!one_pass) {
+          float mx[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx[r] = -INFINITY;
+          if (raw) {
+#pragma unroll
+            for (int c = 0; c < kBN / 32; c += 2) {
+              float xa[32], xb[32];
+              tc::ld32(sbuf + c * 32, xa);
+              tc::ld32(sbuf + (c + 1) * 32, xb);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                mx[i & 3] = tc::max3(mx[i & 3], xa[2 * i], xa[2 * i + 1]);
+                mx[i & 3] = tc::max3(mx[i & 3], xb[2 * i], xb[2 * i + 1]);
+              }
+            }
+          } else {
+            const int vhi = last - kbase;
+#pragma unroll 1
+            for (int c = 0; c < kBN / 32; ++c) {
+              float x[32];
+              tc::ld32(sbuf + c * 32, x);
+              tc::wait_ld();
+              if (p.softcap > 0.f) {
+                // cap tanh(y / cap), tanh(u) = 1 - 2 / (1 + e^(2u))
+                const float two_log2e_over_cap = 2.f * kLog2e / p.softcap, cap_log2e = p.softcap * kLog2e;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  const float e = tc::ex2(fminf(x[i] * qk_scale * two_log2e_over_cap, 126.f));
+                  x[i] = cap_log2e * (1.f - __fdividef(2.f, 1.f + e));
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] *= qk_scale;
+              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = c * 32 + i <= vhi ? x[i] : -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) mx[i & 3] = tc::max3(mx[i & 3], x[2 * i], x[2 * i + 1]);
+              tc::st32(sbuf + c * 32, x);
+            }
+            tc::wait_st();
+          }
+          const float m_tile = tc::max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+          if (!(ok = wait_pv())) break;
+          raise_maximum(raw ? m_tile * qk_scale : m_tile);
+        }
+#pragma unroll 1
+        for (bool again = one_pass;; again = false) {
+          const float scale = raw ? qk_scale : 1.0f;
+          if (kBF16 && !single) {
+            exponentials(scale, std::integral_constant<bool, kBF16>());
+            break;
+          }
+          const float top = exponentials(scale, std::false_type());
+          if (!again || !ok || !__any_sync(0xffffffffu, top > m_run + 8.0f)) break;
+          raise_maximum(top);
+        }
+        if (!ok) break;
         l_run += (ls[0].x + ls[1].x) + (ls[0].y + ls[1].y);
         tc::wait_st();
         tc::fence_before_sync();
         mbar_arrive(&bars.p_full[w]);
       }
       if (!ok) break;
-      if (!wait_warp(&bars.o_done[w], items++)) break;
+      if (!wait_softmax(&bars.o_done[w], items++)) break;
       tc::fence_after_sync();
       const int64_t at = m.slab * a.rows + (int64_t)tok * H + m.kh * g + hl;
       if (row_ok) a.slab_ml[at] = make_float2(m_run, l_run);
