@@ -191,6 +191,37 @@ __device__ __noinline__ void fill_tail_page(uint8_t* stage, const B200SharedPref
   __syncwarp();
 }
 
+// x -> top * tanh(x * to_u), 32 values of a thread; the whole warp.  tanh(u) = u f(u^2) with f a polynomial of
+// degree 6, minimax in relative error over |u| <= 1 (fitted with Lawson's algorithm on 4001
+// Chebyshev-spaced points, 2000 passes; fp32 evaluation within 1.7e-7): 9 packed instructions for two
+// values, where 1 - 2 / (1 + e^(2u)), which takes warps with a larger u, needs two MUFU operations a value.
+__device__ __forceinline__ void soft_cap(float (&x)[32], float to_u, float top) {
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) big = fmaxf(big, fabsf(x[i]));
+  if (__all_sync(0xffffffffu, big * fabsf(to_u) <= 1.f)) {
+    const float coef[7] = {0.99999994f, -0.333328396f, 0.13325204f, -0.0534570292f, 0.0202899799f, -0.00620337902f, 0.0010410226f};
+    const float2 zero = make_float2(0.f, 0.f), scale = make_float2(to_u, to_u), cap = make_float2(top, top);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 u = tc::fma2(make_float2(x[2 * i], x[2 * i + 1]), scale, zero), t = tc::fma2(u, u, zero);
+      float2 f = make_float2(coef[6], coef[6]);
+#pragma unroll
+      for (int k = 5; k >= 0; --k) f = tc::fma2(f, t, make_float2(coef[k], coef[k]));
+      const float2 y = tc::fma2(tc::fma2(u, f, zero), cap, zero);
+      x[2 * i] = y.x;
+      x[2 * i + 1] = y.y;
+    }
+  } else {
+    const float to_e = 2.f * kLog2e * to_u;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float e = tc::ex2(fminf(x[i] * to_e, 126.f));
+      x[i] = top * (1.f - __fdividef(2.f, 1.f + e));
+    }
+  }
+}
+
 template <typename T, int D, bool BESIDE>
 __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) shared_prefix_tc_kernel(const __grid_constant__ SharedPrefixArgs a,
                                                                         const __grid_constant__ SharedPrefixMaps maps) {
@@ -638,13 +669,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
               tc::ld32(sbuf + c * 32, x);
               tc::wait_ld();
               if (p.softcap > 0.f) {
-                // cap tanh(y / cap), tanh(u) = 1 - 2 / (1 + e^(2u))
-                const float two_log2e_over_cap = 2.f * kLog2e / p.softcap, cap_log2e = p.softcap * kLog2e;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const float e = tc::ex2(fminf(x[i] * qk_scale * two_log2e_over_cap, 126.f));
-                  x[i] = cap_log2e * (1.f - __fdividef(2.f, 1.f + e));
-                }
+                soft_cap(x, qk_scale / p.softcap, p.softcap * kLog2e);
               } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] *= qk_scale;

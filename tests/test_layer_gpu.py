@@ -480,6 +480,25 @@ def test_prefix_softcap_scale_sink(d):
     check_prefix(c, scale=-0.1)
 
 
+@pytest.mark.parametrize("cap", [0.5, 3.0, 40.0, 1e4])
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_prefix_softcap_range(d, cap):
+    """Scores far below, around and far above the cap."""
+    c = prefix_case(d, [0, 90, 33, 7], [1, 1, 60, 2], 300, 16, 4, d, scale=2.0, dtype=torch.float16)
+    check_prefix(c, softcap=cap)
+
+
+def test_prefix_many_sequences():
+    """More sequences than a window, a CTA or a scan step covers; some without tokens, some long."""
+    g = np.random.default_rng(5)
+    B = 2600
+    new = [int(x) for x in g.choice([0, 1, 1, 1, 2, 5], B)]
+    new[7], new[1500], new[2599] = 40, 130, 33
+    past = [int(x) for x in g.integers(0, 40, B)]
+    check_prefix(prefix_case(8, past, new, 150, 4, 1, 64))
+    check_prefix(prefix_case(9, past, new, 40, 6, 2, 128))
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [17, 1, 90, 3]])
 def test_prefix_peaked_scores(new):
     """Scores up to about +-600: one key takes all the weight, wherever it lies."""
