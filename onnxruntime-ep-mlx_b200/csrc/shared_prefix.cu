@@ -349,7 +349,9 @@ constexpr int kCopyPairs = 4;  // pairs of query tiles from which the copy of th
 // The shapes the fast path covers; the call also needs 16-byte rows (fast_rows).
 bool fast_shape(const B200SharedPrefixParams& p) {
   return (p.head_size == 64 || p.head_size == 128) && p.block_size % kOwnTile == 0 &&
-         p.num_heads / p.kv_num_heads <= 128;
+         p.num_heads / p.kv_num_heads <= 128 &&
+         // work items are counted in 32 bits: at most 64 ranges and a pair per token, and a pair per sequence
+         ((int64_t)64 * p.num_tokens + p.batch) * p.kv_num_heads < INT32_MAX;
 }
 
 bool fast_rows(const B200SharedPrefixParams& p) {
@@ -406,7 +408,7 @@ size_t layout(const B200SharedPrefixParams& p, int num_sms, SharedPrefixArgs* a)
     return at;
   };
   const size_t d = p.head_size, slabs = (size_t)a->splits + 1, wrows = (size_t)a->own_warps * 2 * a->own_rows;
-  a->next_item = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long)));
+  a->next_item = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t)));
   a->seq_tiles = reinterpret_cast<int*>(take(sizeof(int) * ((size_t)p.batch + 1)));
   a->seq_pairs = reinterpret_cast<int*>(take(sizeof(int) * ((size_t)p.batch + 1)));
   a->token_info = reinterpret_cast<int4*>(take(sizeof(int4) * (size_t)p.num_tokens));

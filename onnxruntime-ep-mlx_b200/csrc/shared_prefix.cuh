@@ -39,7 +39,7 @@ struct SharedPrefixArgs {
   int* seq_pairs;    // [batch + 1] exclusive prefix of query-tile pairs, tensor-core kernel
   int4* token_info;  // [num_tokens] of a token's sequence: first token, tokens (-1: none valid), first
                      // 16-key tile of the own kernel, tiles (0: own keys on the tensor-core kernel)
-  unsigned long long* next_item;  // tensor-core items handed out beyond each CTA's first
+  uint32_t* next_item;  // tensor-core items handed out beyond each CTA's first
   // partials
   float* slab_o;     // [splits + 1][rows][head_size]
   float2* slab_ml;   // [splits + 1][rows]

@@ -117,21 +117,23 @@ struct Item {
   int k_end;                     // prefix: end of the key range
   int n0, n1, n;                 // K/V tiles of query tile 0, 1, and their maximum
   const int32_t* table;
-  int64_t slab;
+  int slab;
 };
 
-// The whole warp.
-__device__ __forceinline__ Item decode_item(const SharedPrefixArgs& a, int64_t it, int64_t prefix_items, int lane) {
+// Item `it` of the list (below 2^31, which the host checked): prefix items ((range, kv head), pair), whose
+// neighbours share their K/V tiles in L2, then chunk items.  The whole warp.
+__device__ __forceinline__ Item decode_item(const SharedPrefixArgs& a, uint32_t it, uint32_t prefix_items, int lane) {
   Item m{};
-  const int KV = a.p.kv_num_heads, TQ = a.tile_tokens;
-  if (it < prefix_items) {  // ((range, kv head), pair): neighbours share their K/V tiles in L2
-    const int pair = (int)(it % a.query_pairs);
-    const int64_t r = it / a.query_pairs;
-    m.kh = (int)(r % KV);
-    m.slab = r / KV;
-    m.tok0 = pair * 2 * TQ;
+  const uint32_t KV = a.p.kv_num_heads;
+  const int TQ = a.tile_tokens;
+  if (it < prefix_items) {
+    const uint32_t r = it / (uint32_t)a.query_pairs, pair = it - r * a.query_pairs;
+    const uint32_t range = r / KV;
+    m.kh = (int)(r - range * KV);
+    m.slab = range;
+    m.tok0 = (int)pair * 2 * TQ;
     m.tok_end = a.p.num_tokens;
-    m.k_lo = (int)m.slab * a.split_tiles * kBN;
+    m.k_lo = (int)range * a.split_tiles * kBN;
     m.k_valid = a.p.prefix_length;
     m.k_end = min(m.k_valid, m.k_lo + a.split_tiles * kBN);
     m.n0 = (m.k_end - m.k_lo + kBN - 1) / kBN;
@@ -141,10 +143,11 @@ __device__ __forceinline__ Item decode_item(const SharedPrefixArgs& a, int64_t i
     return m;
   }
   it -= prefix_items;
-  const int64_t pairs = __ldcg(a.seq_pairs + a.p.batch);
-  const int64_t pair_global = pairs - 1 - it / KV;  // later tiles, which see more keys, first
+  const int pairs = __ldcg(a.seq_pairs + a.p.batch);
+  const int nth = (int)(it / KV);
+  const int pair_global = pairs - 1 - nth;  // later tiles, which see more keys, first
   m.chunk = 1;
-  m.kh = (int)(it % KV);
+  m.kh = (int)(it - nth * KV);
   int lo = 0, hi = a.p.batch;  // the largest lo with seq_pairs[lo] <= pair_global, 32 candidates at a time
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, at = lo + lane * step;
@@ -493,19 +496,19 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
       // ---------------------------------------------------------------- scheduler
       // The first item is the CTA's own and, if it lies in the prefix, needs nothing of the plan, which
       // may still be running then.
-      const int64_t prefix_items = (int64_t)a.splits * p.kv_num_heads * a.query_pairs;
+      const uint32_t prefix_items = (uint32_t)a.splits * p.kv_num_heads * a.query_pairs;
       bool planned = false;
-      int64_t items = 0;
+      uint32_t items = 0;
       for (uint32_t k = 0; !failed_warp(); ++k) {
         const uint32_t slot = k % kSched;
         if (k >= (uint32_t)kSched && !wait_warp(&bars.sched_empty[slot], k / kSched - 1)) break;
-        int64_t it = blockIdx.x;
+        uint32_t it = blockIdx.x;
         if (!planned && (k > 0 || it >= prefix_items)) {
           planned = true;
           // The own kernel needs the plan, not this kernel's results: let it start once the plan is done.
           wait_previous();
           release_dependents();
-          items = prefix_items + (int64_t)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads;
+          items = prefix_items + (uint32_t)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads;
           if (a.v_copy) {
             uint32_t wide = 0;
             for (int i = lane; i < a.copy_ctas; i += 32) wide |= __ldcg(a.v_wide + i);
@@ -517,9 +520,9 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
           }
         }
         if (k > 0) {
-          unsigned long long next = 0;
-          if (lane == 0) next = atomicAdd(a.next_item, 1ull);
-          it = gridDim.x + (int64_t)__shfl_sync(0xffffffffu, next, 0);
+          uint32_t next = 0;
+          if (lane == 0) next = atomicAdd(a.next_item, 1u);
+          it = gridDim.x + __shfl_sync(0xffffffffu, next, 0);
         }
         const bool stop = planned && it >= items;
         Item m{};
@@ -706,7 +709,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
       if (!ok) break;
       if (!wait_softmax(&bars.o_done[w], items++)) break;
       tc::fence_after_sync();
-      const int64_t at = m.slab * a.rows + (int64_t)tok * H + m.kh * g + hl;
+      const int64_t at = (int64_t)m.slab * a.rows + (int64_t)tok * H + m.kh * g + hl;
       if (row_ok) a.slab_ml[at] = make_float2(m_run, l_run);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {

@@ -666,3 +666,35 @@ def test_layer_in_a_graph():
         want, want_res = layer()
         assert torch.equal(got, want) and torch.equal(got_res, want_res)
     del graph
+
+
+def test_example_layer_against_whole_sequences():
+    """The example's last decode step, recomputed from its caches with every sequence's keys in one piece."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "shared_prefix_decode.py")
+    spec = importlib.util.spec_from_file_location("shared_prefix_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    H, KV, d = 8, 2, 128
+    _, got, (layer, x, residual, past, table, ptable, P) = example.serve(batch=5, prefix=203, prompt=20, steps=6, hidden=512,
+                                                                         heads=H, kv_heads=KV, head_size=d)
+    # the step's own keys are in the cache: past counts them after the step
+    codes, scales, _ = skip_rms_norm(x, residual, layer.norm, out_dtype=FP8)
+    qkv = torch._scaled_mm(codes, layer.qkv.t(), scale_a=scales, scale_b=layer.qkv_scale, out_dtype=torch.bfloat16)
+    q = qkv[:, :H * d].double().view(5, H, d)
+    pos = P + past.long() - 1
+    c, s = (t.double()[pos][:, None] for t in (layer.cos, layer.sin))
+    a, b = q[..., :d // 2], q[..., d // 2:]
+    q = torch.cat([a * c - b * s, b * c + a * s], -1).bfloat16().double()
+    out = torch.empty(5, H, d, device="cuda", dtype=torch.float64)
+    for i in range(5):
+        n = int(past[i])
+        rows = [torch.cat([cache[ptable.long()].reshape(-1, KV, d)[:P], cache[table[i].long()].reshape(-1, KV, d)[:n]]).double()
+                for cache in (layer.key_cache, layer.value_cache)]
+        scores = torch.einsum("kgd,skd->kgs", q[i].view(KV, H // KV, d), rows[0]) * d ** -0.5
+        out[i] = torch.einsum("kgs,skd->kgd", scores.softmax(-1), rows[1]).reshape(H, d)
+    want = out.view(5, H * d) @ layer.out.double()
+    # bf16 attention output (2^-9 relative) and bf16 result: 2^-7 of the result's scale
+    assert ((got.double() - want).abs() <= 2.0 ** -7 * want.abs().amax()).all()
