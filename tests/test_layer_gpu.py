@@ -103,6 +103,25 @@ def test_norm_many_rows_and_batch_invariance():
     assert torch.equal(one, out[70000:]) and torch.equal(one_res, res[70000:])
 
 
+@pytest.mark.parametrize("rows,hidden", [(2001, 301), (1500, 2881), (900, 4002), (700, 8191), (650, 12290), (3000, 129)])
+@pytest.mark.parametrize("group", [None, 0, 32, 128])
+def test_norm_many_odd_rows(rows, hidden, group):
+    """Rows off 16 bytes in CTAs that walk: every row, first and last channels included."""
+    g = gen(hidden)
+    x, r, w = normal(g, rows, hidden), normal(g, rows, hidden), normal(g, hidden)
+    s, y = norm64(x, r, w)
+    if group is None:
+        out, res = skip_rms_norm(x, r, w)
+        close16(out, y, y.abs() * 2.0 ** -17)
+        keep = x.clone(), r.clone()
+        skip_rms_norm(keep[0], keep[1], w, output=keep[0], residual_output=keep[1])
+        assert torch.equal(keep[0], out) and torch.equal(keep[1], res)
+    else:
+        codes, scales, res = skip_rms_norm(x, r, w, out_dtype=FP8, group_size=group)
+        check_codes(codes, scales, y, group)
+    close16(res, s, s.abs() * 2.0 ** -23)
+
+
 @pytest.mark.parametrize("pad,shift", [(8, 0), (1, 0), (4, 4), (0, 1), (3, 2)])
 def test_norm_strides_alignment_and_in_place(pad, shift):
     g = gen(pad + 10 * shift)
