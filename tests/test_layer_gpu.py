@@ -103,7 +103,8 @@ def test_norm_many_rows_and_batch_invariance():
     assert torch.equal(one, out[70000:]) and torch.equal(one_res, res[70000:])
 
 
-@pytest.mark.parametrize("rows,hidden", [(2001, 301), (1500, 2881), (900, 4002), (700, 8191), (650, 12290), (3000, 129)])
+@pytest.mark.parametrize("rows,hidden", [(2001, 301), (1500, 2881), (900, 4002), (700, 8191), (650, 12290), (3000, 129), (900, 1031), (700, 256), (700, 1024),
+                                         (650, 16391), (1300, 15), (601, 8200)])
 @pytest.mark.parametrize("group", [None, 0, 32, 128])
 def test_norm_many_odd_rows(rows, hidden, group):
     """Rows off 16 bytes in CTAs that walk: every row, first and last channels included."""
