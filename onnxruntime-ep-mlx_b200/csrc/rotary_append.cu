@@ -4,12 +4,17 @@
 //   pair (x0, x1) -> (x0 c - x1 s, x1 c + x0 s) in fp32, rounded once; c, s from row
 //   position[axis of the pair] of the tables
 //
-// Memory bound: every query, key and value row is read once and written once.
+// Memory bound: every query, key and value row is read once and written once.  Measured, bf16, 128-wide
+// heads: 8192 tokens of 32 + 8 + 8 heads with three axes 42 us (201 MB, 0.73 of 6.5 TB/s), 4096 tokens of
+// 64 + 8 + 8 heads into an fp8 cache 36 us (160 MB, 0.68), 1001 tokens of 14 + 2 + 2 heads of 64 channels
+// 5.4 us, 64 tokens 3.0 us.  The search for later tokens with the same slot is 3.3, 2.4, 1.0 and 0.5 us
+// of these; a table filled first costs two launches more.
 //
 // rotary_append_vec_kernel: a thread owns a unit of 16 channels (two 16-byte pieces: the two halves
 // of 8 rotary pairs, or 16 channels that do not turn) and walks the token's heads with it.  The cos and
 // sin values of a CTA's tokens, gathered once per pair (axes may change anywhere between pairs), wait in
-// shared memory and stay in registers over the heads.  rotary_append_kernel takes what is not aligned to such units.
+// shared memory and stay in registers over the heads; the loads of a token's next heads are in flight as
+// one is stored (1001 tokens: 6.7 us when they went out in batches).  rotary_append_kernel takes what is not aligned to such units.
 //
 // Of several tokens with one slot the last is stored.  Up to B200_ROTARY_APPEND_SCAN_TOKENS tokens,
 // a CTA compares its tokens' slots with every later one (up to 4 tokens per CTA share the reads of
@@ -273,7 +278,7 @@ __device__ __forceinline__ void turn(bool interleaved, const float (&c)[8], cons
 
 // CTA: TOKENS tokens x heads [blockIdx.y * cta_heads, + cta_heads) of the query, key and value heads in
 // that order.  A warp owns one token; a lane owns (unit of `units`, head offset), lanes past the last
-// whole head idle.  kBatch heads' loads go out before the first of them is used.
+// whole head idle.  kBatch heads' loads are in flight: as one is stored, the load kBatch heads on goes out.
 template <typename T, bool FP8, int TOKENS>
 __global__ void __launch_bounds__(kVecThreads, 5) rotary_append_vec_kernel(const __grid_constant__ B200RotaryAppendParams p,
                                                                             const int* keys, const int* last,
@@ -302,19 +307,18 @@ __global__ void __launch_bounds__(kVecThreads, 5) rotary_append_vec_kernel(const
   const int64_t t = t0 + i;
   const bool active = t < p.num_tokens && lane / units < warp_heads;
   const T* q = static_cast<const T*>(p.query) + t * p.query_row_stride;
-  const int q_end = active ? min(H, h_end) : 0;
+  const T* krow = static_cast<const T*>(p.key) + t * p.key_row_stride;
+  const T* vrow = static_cast<const T*>(p.value) + t * p.value_row_stride;
   uint4 xa[kBatch], xb[kBatch];
-  auto load_queries = [&](int h0) {
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int h = h0 + k * head_step;
-      if (h < q_end) {
-        xa[k] = *reinterpret_cast<const uint4*>(q + h * d + ca);
-        xb[k] = *reinterpret_cast<const uint4*>(q + h * d + cb);
-      }
-    }
+  auto load = [&](int k, int h) {
+    const bool value = h >= H + KV;
+    const T* row = h < H ? q + h * d : value ? vrow + (h - H - KV) * d : krow + (h - H) * d;
+    xa[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit : ca));
+    xb[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit + 8 : cb));
   };
-  load_queries(h_first);  // in flight during the gather and the search below
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k)  // in flight during the gather and the search below
+    if (active && h_first + k * head_step < h_end) load(k, h_first + k * head_step);
   extern __shared__ float turns_s[];  // cos [TOKENS][half], sin [TOKENS][half]
   load_turns<T, TOKENS>(p, t0, half, turns_s, turns_s + TOKENS * half);
   int32_t slot = -1;
@@ -346,12 +350,17 @@ __global__ void __launch_bounds__(kVecThreads, 5) rotary_append_vec_kernel(const
     }
   }
   T* out = static_cast<T*>(p.output) + t * p.output_row_stride;
-  for (int h0 = h_first; h0 < q_end;) {
+  const int64_t at = (int64_t)slot * KV * d;  // cache row of the token
+  // the rows that go out as they are or turned: all, or the queries beside an fp8 cache
+  const int end = keep && !FP8 ? h_end : min(H, h_end);
+  int h0 = h_first;
+  for (; h0 < end; h0 += kBatch * head_step) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int h = h0 + k * head_step;
-      if (h >= q_end) break;
-      if (turns) {
+      if (h >= end) break;
+      const bool value = h >= H + KV;
+      if (turns && !value) {
         float a[8], b[8];
         unpack8<T>(xa[k], a);
         unpack8<T>(xb[k], b);
@@ -359,55 +368,38 @@ __global__ void __launch_bounds__(kVecThreads, 5) rotary_append_vec_kernel(const
         xa[k] = pack8<T>(a);
         xb[k] = pack8<T>(b);
       }
-      *reinterpret_cast<uint4*>(out + h * d + ca) = xa[k];
-      *reinterpret_cast<uint4*>(out + h * d + cb) = xb[k];
+      T* row = h < H ? out + h * d : static_cast<T*>(value ? p.value_cache : p.key_cache) + at + (h - H - (value ? KV : 0)) * d;
+      *reinterpret_cast<uint4*>(row + (value ? 16 * unit : ca)) = xa[k];
+      *reinterpret_cast<uint4*>(row + (value ? 16 * unit + 8 : cb)) = xb[k];
+      if (h + kBatch * head_step < end) load(k, h + kBatch * head_step);
     }
-    h0 += kBatch * head_step;
-    load_queries(h0);
   }
-  if (!keep) return;
-  // this lane's first key or value head
-  int h0 = h_first + (h_first < H ? (H - h_first + head_step - 1) / head_step * head_step : 0);
-  const T* krow = static_cast<const T*>(p.key) + t * p.key_row_stride;
-  const T* vrow = static_cast<const T*>(p.value) + t * p.value_row_stride;
-  const int64_t at = (int64_t)slot * KV * d;  // cache row of the token
-  for (; h0 < h_end; h0 += kBatch * head_step) {
-    float scale[kBatch];
+  if constexpr (FP8) {  // in batches of their own: the divisions leave no registers for more (39 against 36 us)
+    if (!keep) return;
+    h0 = h_first + (h_first < H ? (H - h_first + head_step - 1) / head_step * head_step : 0);
+    const float* k_scale = p.k_scale + (int64_t)(slot / p.block_size) * KV;
+    const float* v_scale = p.v_scale + (int64_t)(slot / p.block_size) * KV;
+    for (; h0 < h_end; h0 += kBatch * head_step) {
+      float scale[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int kh = h0 + k * head_step - H;
-      if (kh + H >= h_end) break;
-      const bool value = kh >= KV;
-      const T* row = value ? vrow + (kh - KV) * d : krow + kh * d;
-      xa[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit : ca));
-      xb[k] = *reinterpret_cast<const uint4*>(row + (value ? 16 * unit + 8 : cb));
-      if constexpr (FP8)
-        scale[k] = __ldg((value ? p.v_scale - KV : p.k_scale) + (int64_t)(slot / p.block_size) * KV + kh);
-    }
+      for (int k = 0; k < kBatch; ++k) {
+        const int h = h0 + k * head_step;
+        if (h >= h_end) break;
+        load(k, h);
+        scale[k] = __ldg(h >= H + KV ? v_scale + (h - H - KV) : k_scale + (h - H));
+      }
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int kh = h0 + k * head_step - H;
-      if (kh + H >= h_end) break;
-      const bool value = kh >= KV;
-      const int64_t row = at + (value ? kh - KV : kh) * d;
-      const int sa = value ? 16 * unit : ca, sb = value ? 16 * unit + 8 : cb;
-      void* cache = value ? p.value_cache : p.key_cache;
-      float a[8], b[8];
-      if (FP8 || (turns && !value)) {
+      for (int k = 0; k < kBatch; ++k) {
+        const int h = h0 + k * head_step;
+        if (h >= h_end) break;
+        const bool value = h >= H + KV;
+        float a[8], b[8];
         unpack8<T>(xa[k], a);
         unpack8<T>(xb[k], b);
-      }
-      if (turns && !value) turn(interleaved, c, s, a, b);
-      if constexpr (FP8) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + row + sa) = e4m3x8(a, scale[k]);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + row + sb) = e4m3x8(b, scale[k]);
-      } else {
-        if (turns && !value) {
-          xa[k] = pack8<T>(a);
-          xb[k] = pack8<T>(b);
-        }
-        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + row + sa) = xa[k];
-        *reinterpret_cast<uint4*>(static_cast<T*>(cache) + row + sb) = xb[k];
+        if (turns && !value) turn(interleaved, c, s, a, b);
+        uint8_t* row = static_cast<uint8_t*>(value ? p.value_cache : p.key_cache) + at + (h - H - (value ? KV : 0)) * d;
+        *reinterpret_cast<uint2*>(row + (value ? 16 * unit : ca)) = e4m3x8(a, scale[k]);
+        *reinterpret_cast<uint2*>(row + (value ? 16 * unit + 8 : cb)) = e4m3x8(b, scale[k]);
       }
     }
   }
