@@ -130,7 +130,13 @@ B200_API int b200_rotary_append(const B200RotaryAppendParams* p, void* stream);
  * included, are read from the caches (b200_rotary_append or b200_kv_append first).
  * Scores are scale * q.k, soft-capped as softcap * tanh(score / softcap) when softcap > 0; the
  * optional head_sink adds exp(sink[h]) to each softmax denominator.  Softmax and sums are fp32.
- * Pages may hold anything in slots past a sequence's (or the prefix's) last key.
+ * Pages may hold anything in slots past a sequence's (or the prefix's) last key.  A NaN in a query or
+ * in a key makes the rows that see it NaN, and no others.  The values of a call's new tokens should be
+ * finite: hidden ones are multiplied with a weight of zero, so an infinity or NaN in the value of a new
+ * token can reach earlier tokens of the same sequence in the call.
+ * Head sizes 64 and 128 with a block_size that is a multiple of 16, at most 128 query heads per kv head
+ * and 16-byte aligned rows run on the tensor cores; everything else, up to head size 256, runs in a
+ * plain kernel that reads the prefix again for every token and head.
  * Invalid metadata (lengths, table capacity, block ids) sets bits of *device_status; the rows it
  * concerns are unspecified, nothing outside the tensors is read or written.
  */
@@ -163,7 +169,10 @@ typedef struct B200SharedPrefixParams {
 } B200SharedPrefixParams;
 
 /* Bytes of device workspace (shapes and prefix_length only).  A workspace serves one call in
- * flight. */
+ * flight.  Most of it holds fp32 partial outputs: num_tokens * num_heads * (head_size + 2) floats for the
+ * own keys and for each range that the prefix is split into (up to 64 with few tokens, one or two with
+ * many), 15 to 29 MB for cut own keys, and for bf16 calls of many tokens an fp16 copy of the prefix's
+ * values. */
 B200_API int b200_shared_prefix_attention_workspace_size(const B200SharedPrefixParams* p, size_t* bytes);
 B200_API int b200_shared_prefix_attention(const B200SharedPrefixParams* p, void* stream);
 

@@ -5,9 +5,9 @@
 // Softmax over a union of key sets: with M the largest m of a row's triples (m, l, o),
 //   out = sum 2^(m_i - M) o_i / (sum 2^(m_i - M) l_i + 2^(sink log2 e - M))
 //
-// shared_prefix_generic_kernel (any head size up to 256, block size and head ratio): a CTA per (token, query head); its warps take every kWarps-th key
-// of the prefix and of the token's own keys with an fp32 running softmax (m, l, o), and the warps'
-// triples are joined in shared memory.
+// shared_prefix_generic_kernel (any head size up to 256, block size, head ratio and alignment): a CTA per
+// (token, query head); its warps take the keys of the prefix and the token's own four at a time with an
+// fp32 running softmax (m, l, o), and the warps' triples are joined in shared memory.
 #include <algorithm>
 #include <cmath>
 
@@ -100,14 +100,16 @@ __global__ void __launch_bounds__(32 * kGenericWarps) shared_prefix_generic_kern
   float top = sink;
   for (int w = 0; w < kGenericWarps; ++w) top = fmaxf(top, part_m[w]);
   float sum = p.head_sink ? expf(sink - top) : 0.f;
-  for (int w = 0; w < kGenericWarps; ++w)
+  for (int w = 0; w < kGenericWarps; ++w) {
     if (part_m[w] != -INFINITY) sum += part_l[w] * expf(part_m[w] - top);
+    else if (part_l[w] != part_l[w]) sum = part_l[w];  // NaN scores only
+  }
   T* out = static_cast<T*>(p.output) + t * p.output_row_stride + (int64_t)h * d;
   for (int c = threadIdx.x; c < d; c += blockDim.x) {
     float acc = 0.f;
     for (int w = 0; w < kGenericWarps; ++w)
       if (part_m[w] != -INFINITY) acc += part_o[w][c] * expf(part_m[w] - top);
-    out[c] = act<T>::from_f(sum > 0.f ? acc / sum : 0.f);
+    out[c] = act<T>::from_f(sum == 0.f ? 0.f : acc / sum);
   }
 }
 
@@ -303,6 +305,9 @@ __global__ void __launch_bounds__(kMergeThreads) shared_prefix_merge_kernel(cons
     float m = top;
 #pragma unroll
     for (int j = 0; j < kMergeBatch; ++j) m = fmaxf(m, ml[j].x);
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j)
+      if (ml[j].y != ml[j].y) sum = ml[j].y;  // NaN scores only: m has stayed at its start
     if (m == -INFINITY) continue;
     const float f = exp2f(top - m);
     top = m;
@@ -466,7 +471,7 @@ cudaError_t launch_shared_prefix(const B200SharedPrefixParams& p, int num_sms, c
   shared_prefix_plan_kernel<<<1 + a.copy_ctas, kPlanThreads, 0, stream>>>(a);
   e = cudaGetLastError();
   if (e == cudaSuccess) e = launch_shared_prefix_tc(a, maps, num_sms, stream);
-  if (e == cudaSuccess) e = launch_shared_prefix_own(a, maps, stream);
+  if (e == cudaSuccess) e = launch_shared_prefix_own(a, stream);
   if (e == cudaSuccess)
     e = p.act_dtype == B200_DTYPE_BFLOAT16 ? launch_merge_t<__nv_bfloat16>(a, stream) : launch_merge_t<__half>(a, stream);
   if (e == cudaSuccess) add_launches(4);

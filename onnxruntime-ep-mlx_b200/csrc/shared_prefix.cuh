@@ -60,7 +60,7 @@ constexpr int kPrefixKeys = 128;  // keys per tile of the tensor-core kernel
 
 cudaError_t launch_shared_prefix_tc(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms,
                                     cudaStream_t stream);
-cudaError_t launch_shared_prefix_own(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, cudaStream_t stream);
+cudaError_t launch_shared_prefix_own(const SharedPrefixArgs& a, cudaStream_t stream);
 
 // Stream-K ranges of the own kernel: T tiles over W warps, the first `extra` warps own `each` + 1
 // consecutive tiles and the others `each`.

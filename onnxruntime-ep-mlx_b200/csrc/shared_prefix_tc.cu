@@ -194,6 +194,19 @@ __device__ __noinline__ void fill_tail_page(uint8_t* stage, const B200SharedPref
   __syncwarp();
 }
 
+// Maxima that keep a NaN: a row whose scores hold one has to end as NaN, and the exponential on the FMA pipe
+// alone would drop it.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // x -> top * tanh(x * to_u), 32 values of a thread; the whole warp.  tanh(u) = u f(u^2) with f a polynomial of
 // degree 6, minimax in relative error over |u| <= 1 (fitted with Lawson's algorithm on 4001
 // Chebyshev-spaced points, 2000 passes; fp32 evaluation within 1.7e-7): 9 packed instructions for two
@@ -219,7 +232,7 @@ __device__ __forceinline__ void soft_cap(float (&x)[32], float to_u, float top) 
     const float to_e = 2.f * kLog2e * to_u;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const float e = tc::ex2(fminf(x[i] * to_e, 126.f));
+      const float e = tc::ex2(min_nan(x[i] * to_e, 126.f));
       x[i] = top * (1.f - __fdividef(2.f, 1.f + e));
     }
   }
@@ -590,7 +603,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
             uint32_t hi[16], lo[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              if (D == 64 && !decltype(as_pair)::value) mx[i & 1] = tc::max3(mx[i & 1], x[2 * i], x[2 * i + 1]);
+              if (D == 64 && !decltype(as_pair)::value) mx[i & 1] = max3_nan(mx[i & 1], x[2 * i], x[2 * i + 1]);
               const float2 e = tc::fma2(make_float2(x[2 * i], x[2 * i + 1]), ks2, nmu2);
               const float2 pr = kPolyEvery > 0 && i % (kPolyEvery > 0 ? kPolyEvery : 1) == kPolyEvery - 1 ? tc::exp2_poly2(e) : make_float2(tc::ex2(e.x), tc::ex2(e.y));
               ls[i & 1] = tc::add2(ls[i & 1], pr);
@@ -620,10 +633,11 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
             chunk(xb, c + 1);
             tc::wait_ld();
           }
-          return fmaxf(mx[0], mx[1]) * scale;
+          return max3_nan(mx[0], mx[1], mx[1]) * scale;
         };
         // The running maximum takes in `m_tile`, and O and l follow, where it grows by more than 2^8.
         auto raise_maximum = [&](float m_tile) {
+          if (!(m_tile < INFINITY)) l_run = NAN;  // a NaN or +inf among the row's scores
           const float m_new = fmaxf(m_run, m_tile);
           const bool grow = m_new > m_run + 8.0f;
           const float alpha = (grow && m_run != -INFINITY) ? tc::ex2(m_run - m_new) : 1.0f;
@@ -660,8 +674,8 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
               tc::wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                mx[i & 3] = tc::max3(mx[i & 3], xa[2 * i], xa[2 * i + 1]);
-                mx[i & 3] = tc::max3(mx[i & 3], xb[2 * i], xb[2 * i + 1]);
+                mx[i & 3] = max3_nan(mx[i & 3], xa[2 * i], xa[2 * i + 1]);
+                mx[i & 3] = max3_nan(mx[i & 3], xb[2 * i], xb[2 * i + 1]);
               }
             }
           } else {
@@ -680,12 +694,12 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
 #pragma unroll
               for (int i = 0; i < 32; ++i) x[i] = c * 32 + i <= vhi ? x[i] : -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) mx[i & 3] = tc::max3(mx[i & 3], x[2 * i], x[2 * i + 1]);
+              for (int i = 0; i < 16; ++i) mx[i & 3] = max3_nan(mx[i & 3], x[2 * i], x[2 * i + 1]);
               tc::st32(sbuf + c * 32, x);
             }
             tc::wait_st();
           }
-          const float m_tile = tc::max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+          const float m_tile = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
           if (!(ok = wait_pv())) break;
           raise_maximum(raw ? m_tile * qk_scale : m_tile);
         }
@@ -697,6 +711,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
             break;
           }
           const float top = exponentials(scale, std::false_type());
+          if (!(top < INFINITY)) l_run = NAN;
           if (!again || !ok || !__any_sync(0xffffffffu, top > m_run + 8.0f)) break;
           raise_maximum(top);
         }

@@ -500,6 +500,42 @@ def test_prefix_softcap_scale_sink(d):
     check_prefix(c, scale=-0.1)
 
 
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("B", [5, 140])
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_prefix_nan_scores(d, B, softcap):
+    """A NaN in a query, in a key of the prefix or in an own key: NaN in the rows that see it, in no other."""
+    H, KV, P = 16, 2, 300
+    new = [1] * (B - 2) + [3, 40]
+    c = prefix_case(d, [4] * B, new, P, H, KV, d)
+    clean = prefix_call(c, softcap=softcap).view(-1, H, d)
+    q, kc = c["q"].clone(), c["kc"].clone()
+    c["q"].view(-1, H, d)[2, 5, 7] = float("nan")
+    touched = torch.zeros(clean.shape[0], H, dtype=torch.bool, device="cuda")
+    touched[2, 5] = True
+    def check():
+        got = prefix_call(c, softcap=softcap).view(-1, H, d)
+        assert torch.isnan(got[touched]).all()
+        # the running maxima of other rows may have moved at other tiles: a unit of the output type
+        torch.testing.assert_close(got[~touched], clean[~touched], rtol=2.0 ** -7, atol=1e-3)
+    check()
+    c["q"].copy_(q)
+    for b, at, first in ((0, 3, 0), (1, 4, 1), (B - 2, 5, B - 1), (B - 1, 20, B + 17)):  # own key `at`, seen from token `first` on
+        slot = int(c["table"][b][at // 16]) * 16 + at % 16
+        c["kc"].view(-1, KV, d)[slot, 1, 3] = float("nan")
+        touched.zero_()
+        touched[first:len(touched) if b == B - 1 else first + (2 if b == B - 2 else 1), H // 2:] = True
+        check()
+        c["kc"].copy_(kc)
+    for at in (0, 14, 15, 30, 31, 100, 127, 128, 299):
+        slot = int(c["ptable"][at // 16]) * 16 + at % 16
+        c["kc"].view(-1, KV, d)[slot, 1, 3] = float("nan")
+        touched.zero_()
+        touched[:, H // 2:] = True
+        check()
+        c["kc"].copy_(kc)
+
+
 @pytest.mark.parametrize("cap", [0.5, 3.0, 40.0, 1e4])
 @pytest.mark.parametrize("d", [64, 128, 80])
 def test_prefix_softcap_range(d, cap):
