@@ -7,14 +7,15 @@
 // Memory bound: every query, key and value row is read once and written once.  Measured, bf16, 128-wide
 // heads: 8192 tokens of 32 + 8 + 8 heads with three axes 42 us (201 MB, 0.73 of 6.5 TB/s), 4096 tokens of
 // 64 + 8 + 8 heads into an fp8 cache 36 us (160 MB, 0.68), 1001 tokens of 14 + 2 + 2 heads of 64 channels
-// 5.4 us, 64 tokens 3.0 us.  The search for later tokens with the same slot is 3.3, 2.4, 1.0 and 0.5 us
+// 5.4 us, 128 tokens 3.0 us.  The search for later tokens with the same slot is 3.3, 2.4, 1.0 and 0.5 us
 // of these; a table filled first costs two launches more.
 //
 // rotary_append_vec_kernel: a thread owns a unit of 16 channels (two 16-byte pieces: the two halves
 // of 8 rotary pairs, or 16 channels that do not turn) and walks the token's heads with it.  The cos and
 // sin values of a CTA's tokens, gathered once per pair (axes may change anywhere between pairs), wait in
 // shared memory and stay in registers over the heads; the loads of a token's next heads are in flight as
-// one is stored (1001 tokens: 6.7 us when they went out in batches).  rotary_append_kernel takes what is not aligned to such units.
+// one is stored (1001 tokens: 6.7 us when they went out in batches).  rotary_append_kernel takes what is
+// not aligned to such units.
 //
 // Of several tokens with one slot the last is stored.  Up to B200_ROTARY_APPEND_SCAN_TOKENS tokens,
 // a CTA compares its tokens' slots with every later one (up to 4 tokens per CTA share the reads of
