@@ -467,26 +467,33 @@ __global__ void __launch_bounds__(max_threads(OWNER), min_ctas(OWNER, ITEMS))
         }
       }
       sync_row<OWNER>();
-      for (int i = tid; i < groups; i += threads) scales[i] = scale_of(__int_as_float(group_max[i]));
+      if (!p.group_size) {
+        const float scale = scale_of(__int_as_float(group_max[0])), inv = inverse(scale);
+        if (tid == 0) scales[0] = scale;
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k) {
-        const int e = first(k);
-        if (!valid(k)) continue;
-        const int g0 = e >> group_log2, next = (g0 + 1 << group_log2) - e;
-        const float inv = inverse(scale_of(__int_as_float(group_max[g0])));
-        if (p.group_size == 0 || next >= 8) {
-          scale_by<8>(s[k], inv);
-        } else {
-          const float inv1 = inverse(scale_of(__int_as_float(group_max[g0 + 1])));
+        for (int k = 0; k < ITEMS; ++k) scale_by<8>(s[k], inv);
+        s1[0] *= inv;
+      } else {
+        for (int i = tid; i < groups; i += threads) scales[i] = scale_of(__int_as_float(group_max[i]));
 #pragma unroll
-          for (int j = 0; j < 8; ++j) s[k][j] *= j < next ? inv : inv1;
+        for (int k = 0; k < ITEMS; ++k) {
+          if (!valid(k)) continue;
+          const int g0 = first(k) >> group_log2, next = (g0 + 1 << group_log2) - first(k);
+          const float inv = inverse(scale_of(__int_as_float(group_max[g0])));
+          if (next >= 8) {
+            scale_by<8>(s[k], inv);
+          } else {
+            const float inv1 = inverse(scale_of(__int_as_float(group_max[g0 + 1])));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[k][j] *= j < next ? inv : inv1;
+          }
         }
-        store_e4m3<8>(out + e, s[k]);
+        if (single) s1[0] *= inverse(scale_of(__int_as_float(group_max[es >> group_log2])));
       }
-      if (single) {
-        s1[0] *= inverse(scale_of(__int_as_float(group_max[es >> group_log2])));
-        store_e4m3<1>(out + es, s1);
-      }
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        if (valid(k)) store_e4m3<8>(out + first(k), s[k]);
+      if (single) store_e4m3<1>(out + es, s1);
     }
   }
 }
