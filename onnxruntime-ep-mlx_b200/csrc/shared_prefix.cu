@@ -246,14 +246,16 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Merge: D / 4 lanes per (token, head) row join the row's triples, kMergeBatch of them in flight.
-// Bound by the slabs' reads, which come from L2 as far as the own keys' stream has left them there.
+// Merge: D / 4 lanes per (token, head) row join the row's triples, BATCH of them in flight.  Bound by the
+// slabs' reads, which come from L2 as far as the own keys' stream has left them there, and by the issue of
+// instructions: batches of 4 where a row has few triples (whole calls with 4 and 8: 4000 tokens and at most
+// 3 ranges 214 against 218 us, 256 tokens 335 against 338; 128 tokens and 9 ranges 89.7 against 89.0).
 // ---------------------------------------------------------------------------------------------
 constexpr int kMergeThreads = 128;
-constexpr int kMergeBatch = 8;
+constexpr int kFewRanges = 3;
 constexpr float kLog2eMerge = 1.4426950408889634f;
 
-template <typename T, int D>
+template <typename T, int D, int BATCH>
 __global__ void __launch_bounds__(kMergeThreads) shared_prefix_merge_kernel(const SharedPrefixArgs a, int vector_rows) {
   constexpr int kLanes = D / 4;
   const B200SharedPrefixParams& p = a.p;
@@ -287,11 +289,11 @@ __global__ void __launch_bounds__(kMergeThreads) shared_prefix_merge_kernel(cons
     sum = 1.f;
   }
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = 0; base < parts; base += kMergeBatch) {
-    float2 ml[kMergeBatch];
-    float4 o[kMergeBatch];
+  for (int base = 0; base < parts; base += BATCH) {
+    float2 ml[BATCH];
+    float4 o[BATCH];
 #pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) {
+    for (int j = 0; j < BATCH; ++j) {
       const int i = base + j, piece = i - a.splits;
       ml[j] = make_float2(-INFINITY, 0.f);
       if (i < parts) {
@@ -304,9 +306,9 @@ __global__ void __launch_bounds__(kMergeThreads) shared_prefix_merge_kernel(cons
     }
     float m = top;
 #pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) m = fmaxf(m, ml[j].x);
+    for (int j = 0; j < BATCH; ++j) m = fmaxf(m, ml[j].x);
 #pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j)
+    for (int j = 0; j < BATCH; ++j)
       if (ml[j].y != ml[j].y) sum = ml[j].y;  // NaN scores only: m has stayed at its start
     if (m == -INFINITY) continue;
     const float f = exp2f(top - m);
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(kMergeThreads) shared_prefix_merge_kernel(cons
     sum *= f;
     acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
 #pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) {
+    for (int j = 0; j < BATCH; ++j) {
       if (ml[j].x == -INFINITY) continue;
       const float w = exp2f(ml[j].x - m);
       sum += ml[j].y * w;
@@ -338,8 +340,10 @@ cudaError_t launch_merge_t(const SharedPrefixArgs& a, cudaStream_t stream) {
   const bool vec = (reinterpret_cast<uintptr_t>(a.p.output) | (uintptr_t)(a.p.output_row_stride * 2)) % 8 == 0;
   const int64_t per_cta = kMergeThreads / (a.p.head_size / 4);
   const dim3 grid((unsigned)((a.rows + per_cta - 1) / per_cta)), block(kMergeThreads);
-  return a.p.head_size == 64 ? launch_dependent(shared_prefix_merge_kernel<T, 64>, grid, block, 0, stream, a, (int)vec)
-                             : launch_dependent(shared_prefix_merge_kernel<T, 128>, grid, block, 0, stream, a, (int)vec);
+  auto kernel = a.p.head_size == 64
+                    ? (a.splits <= kFewRanges ? shared_prefix_merge_kernel<T, 64, 4> : shared_prefix_merge_kernel<T, 64, 8>)
+                    : (a.splits <= kFewRanges ? shared_prefix_merge_kernel<T, 128, 4> : shared_prefix_merge_kernel<T, 128, 8>);
+  return launch_dependent(kernel, grid, block, 0, stream, a, (int)vec);
 }
 
 // ---------------------------------------------------------------------------------------------
