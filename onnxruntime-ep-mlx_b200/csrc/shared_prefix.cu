@@ -127,7 +127,8 @@ void launch_generic_t(const B200SharedPrefixParams& p, cudaStream_t stream) {
 // where launched, copy the prefix's bf16 values to fp16 [key][kv head][channel]: with fp16 values the
 // tensor-core pass can carry P as one fp16 value instead of a bf16 hi + lo pair, which takes a third of
 // its MMA work.  The conversion is exact from 2^-14 up to 65504 (below, within 2^-25); a CTA that meets
-// anything beyond, or a NaN, says so and the tensor-core pass then reads the bf16 pages.
+// anything beyond, or a NaN, says so and the tensor-core pass then reads the bf16 pages.  128 sequences 5 us;
+// the copy of 16384 keys of 8 heads of 128 channels 16 us (67 MB).  The tensor-core pass starts beside both.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
