@@ -130,6 +130,8 @@ B200_API int b200_rotary_append(const B200RotaryAppendParams* p, void* stream);
  * included, are read from the caches (b200_rotary_append or b200_kv_append first).
  * Scores are scale * q.k, soft-capped as softcap * tanh(score / softcap) when softcap > 0; the
  * optional head_sink adds exp(sink[h]) to each softmax denominator.  Softmax and sums are fp32.
+ * For their product with the values the weights are rounded to fp16 or carried as two bf16 parts; the
+ * values enter as they are stored, whatever their magnitude.
  * Pages may hold anything in slots past a sequence's (or the prefix's) last key.  A NaN in a query or
  * in a key makes the rows that see it NaN, and no others.  The values of a call's new tokens should be
  * finite: hidden ones are multiplied with a weight of zero, so an infinity or NaN in the value of a new

@@ -126,8 +126,10 @@ void launch_generic_t(const B200SharedPrefixParams& p, cudaStream_t stream) {
 // Plan: CTA 0 checks the lengths, routes every sequence and lays out both work lists.  The other CTAs,
 // where launched, copy the prefix's bf16 values to fp16 [key][kv head][channel]: with fp16 values the
 // tensor-core pass can carry P as one fp16 value instead of a bf16 hi + lo pair, which takes a third of
-// its MMA work.  The conversion is exact from 2^-14 up to 65504 (below, within 2^-25); a CTA that meets
-// anything beyond, or a NaN, says so and the tensor-core pass then reads the bf16 pages.  128 sequences 5 us;
+// its MMA work.  The copy is exact or not used: values go in times kCopyScale, which fp16 holds to the last
+// bit for magnitudes from 2^-28 to below 32 and for zero (2^11 puts that window around values of order 0.01
+// to 10); a CTA that meets any other value names its kv head, and the tensor-core pass reads that head's
+// values from the bf16 pages.  128 sequences 5 us;
 // the copy of 16384 keys of 8 heads of 128 channels 16 us (67 MB).  The tensor-core pass starts beside both.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
@@ -171,7 +173,10 @@ __device__ __forceinline__ void copy_prefix_values(const SharedPrefixArgs& a) {
   const B200SharedPrefixParams& p = a.p;
   const int64_t vecs = (int64_t)p.kv_num_heads * p.head_size / 8;  // 16-byte pieces of one key's values
   const int64_t n = vecs * p.prefix_length, step = (int64_t)a.copy_ctas * kPlanThreads;
-  uint32_t over = 0;
+  __shared__ unsigned long long inexact_heads;
+  if (threadIdx.x == 0) inexact_heads = 0;
+  __syncthreads();
+  unsigned long long inexact = 0;
 #pragma unroll 4
   for (int64_t i = (int64_t)(blockIdx.x - 1) * kPlanThreads + threadIdx.x; i < n; i += step) {
     const int64_t key = i / vecs;
@@ -180,17 +185,21 @@ __device__ __forceinline__ void copy_prefix_values(const SharedPrefixArgs& a) {
     if (blk >= 0 && blk < p.num_blocks)  // the tensor-core kernel reports the others
       v = __ldg(static_cast<const uint4*>(p.value_cache) + ((int64_t)blk * p.block_size + key % p.block_size) * vecs + (i - key * vecs));
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t o[4];
+    uint32_t o[4], outside = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      over |= (w[k] & 0x7fff7fffu) + 0x38803880u;  // bit 15 / 31: bf16 magnitude 0x4780 (65536) and above
-      const __half2 h = __floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+      // bits 15 and 31: a magnitude of 0x4200 (32) and above, or below 0x3180 (2^-28) and not zero
+      const uint32_t m = w[k] & 0x7fff7fffu;
+      outside |= (m + 0x3e003e00u) | (~((m | 0x80008000u) - 0x31803180u) & (m + 0x7fff7fffu));
+      const __half2 h = __floats2half2_rn(__uint_as_float(w[k] << 16) * kCopyScale, __uint_as_float(w[k] & 0xffff0000u) * kCopyScale);
       o[k] = *reinterpret_cast<const uint32_t*>(&h);
     }
+    if (outside & 0x80008000u) inexact |= 1ull << ((uint32_t)(i - key * vecs) / (uint32_t)(p.head_size / 8) & 63u);
     reinterpret_cast<uint4*>(a.v_copy)[i] = make_uint4(o[0], o[1], o[2], o[3]);
   }
-  const int wide = __syncthreads_or((over & 0x80008000u) != 0);
-  if (threadIdx.x == 0) a.v_wide[blockIdx.x - 1] = wide;
+  if (inexact) atomicOr(&inexact_heads, inexact);
+  __syncthreads();
+  if (threadIdx.x == 0) a.v_inexact[blockIdx.x - 1] = inexact_heads;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const SharedPrefixArgs a) {
@@ -428,7 +437,7 @@ size_t layout(const B200SharedPrefixParams& p, int num_sms, SharedPrefixArgs* a)
   a->warp_o = reinterpret_cast<float*>(take(sizeof(float) * wrows * d));
   a->v_copy = nullptr;
   if (copy) {
-    a->v_wide = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * a->copy_ctas));
+    a->v_inexact = reinterpret_cast<uint64_t*>(take(sizeof(uint64_t) * a->copy_ctas));
     a->v_copy = reinterpret_cast<__half*>(take(2 * (size_t)p.prefix_length * p.kv_num_heads * d));
   }
   return off;

@@ -32,7 +32,7 @@ struct SharedPrefixArgs {
   int beside;        // tensor-core CTAs leave room for the own kernel's
   // fp16 copy of the prefix's values (bf16 calls whose copy pays: see shared_prefix_plan_kernel)
   __half* v_copy;    // [prefix_length][kv heads][head_size], or null
-  uint32_t* v_wide;  // [copy_ctas] nonzero: the CTA met a value beyond the fp16 range
+  uint64_t* v_inexact;  // [copy_ctas] kv heads (bit: head % 64) of which the CTA met a value that fp16 does not hold
   int copy_ctas;
   // plan
   int* seq_tiles;    // [batch + 1] exclusive prefix of 16-key tiles (per kv head), own kernel
@@ -57,6 +57,7 @@ constexpr int kOwnTile = 16;  // keys per tile of the own kernel
 constexpr int kOwnWarps = 4;  // warps per CTA
 constexpr int kOwnCtasPerSm = 3;  // its shared memory, 65 KB per CTA, leaves room for three
 constexpr int kPrefixKeys = 128;  // keys per tile of the tensor-core kernel
+constexpr float kCopyScale = 2048.f;  // factor on the values of v_copy, taken out of the pass's results
 
 cudaError_t launch_shared_prefix_tc(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms,
                                     cudaStream_t stream);

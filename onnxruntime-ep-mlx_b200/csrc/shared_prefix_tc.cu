@@ -254,7 +254,8 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) Bars bars;
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int s_failed, s_copy;  // s_copy: prefix items take the values' fp16 copy
+  __shared__ volatile int s_failed;
+  __shared__ volatile uint64_t s_inexact;  // kv heads (bit: head % 64) whose prefix values the fp16 copy does not hold
   __shared__ Item s_items[kSched];
 
   const B200SharedPrefixParams& p = a.p;
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
     if (!a.v_copy || m.chunk) return true;
     if (!plan_seen && !wait(&bars.plan, 0)) return false;
     plan_seen = true;
-    copy = s_copy != 0;
+    copy = !(s_inexact >> (m.kh & 63) & 1);
     return true;
   };
 
@@ -526,11 +527,11 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
           release_dependents();
           items = prefix_items + (uint32_t)__ldcg(a.seq_pairs + p.batch) * p.kv_num_heads;
           if (a.v_copy) {
-            uint32_t wide = 0;
-            for (int i = lane; i < a.copy_ctas; i += 32) wide |= __ldcg(a.v_wide + i);
-            wide = __any_sync(0xffffffffu, wide != 0);
+            uint64_t heads = 0;
+            for (int i = lane; i < a.copy_ctas; i += 32) heads |= __ldcg(reinterpret_cast<const unsigned long long*>(a.v_inexact) + i);
+            const uint32_t low = __reduce_or_sync(0xffffffffu, (uint32_t)heads), high = __reduce_or_sync(0xffffffffu, (uint32_t)(heads >> 32));
             if (lane == 0) {
-              s_copy = !wide;
+              s_inexact = (uint64_t)high << 32 | low;
               mbar_arrive(&bars.plan);
             }
           }
@@ -729,6 +730,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
       tc::fence_after_sync();
       const int64_t at = (int64_t)m.slab * a.rows + (int64_t)tok * H + m.kh * g + hl;
       if (row_ok) a.slab_ml[at] = make_float2(m_run, l_run);
+      const float unscale = copied ? 1.f / kCopyScale : 1.f;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
@@ -737,7 +739,8 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
         if (row_ok) {
           float4* dst = reinterpret_cast<float4*>(a.slab_o + at * D + c * 32);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i)
+            dst[i] = make_float4(o[4 * i] * unscale, o[4 * i + 1] * unscale, o[4 * i + 2] * unscale, o[4 * i + 3] * unscale);
         }
       }
       tc::fence_before_sync();

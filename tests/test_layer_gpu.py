@@ -583,6 +583,36 @@ def test_prefix_values_beyond_fp16(d, value):
         assert not torch.isfinite(got[touched]).any()
 
 
+def weighted_magnitude(c):
+    """sum_j p_j |v_j| of every output channel, in 64 bits."""
+    return prefix64({**c, "vc": c["vc"].abs()})
+
+
+@pytest.mark.parametrize("B", [5, 150])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e-5, 1e-6, 1e-8, 1e-30])
+def test_prefix_small_values(size, d, B):
+    """bf16 values far below 1, with few and with many query tiles: the bound scales with them."""
+    c = prefix_case(d, [3] * B, [1] * B, 400, 16, 2, d)
+    c["vc"] = c["vc"] * size
+    close16(prefix_call(c), prefix64(c), 2e-3 * size)
+
+
+@pytest.mark.parametrize("B", [5, 150])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("by", ["head", "channel", "key"])
+def test_prefix_values_of_mixed_size(by, d, B):
+    """Values whose magnitude differs by kv head, by channel or by key over eight decades, and rows that one key
+    all but fills: the bound, 2e-3 for values of order one, is one on every row's own sum of p |v|."""
+    KV = 4
+    c = prefix_case(d, [3] * B, [1] * B, 400, 16, KV, d, scale=4.0 if by == "key" else 1.0)
+    blocks, bs = c["vc"].shape[:2]
+    shape = dict(head=(1, 1, KV, 1), channel=(1, 1, 1, d), key=(blocks, bs, 1, 1))[by]
+    size = 10.0 ** -(8 * torch.rand(shape, device="cuda", generator=gen(7)))
+    c["vc"] = (c["vc"].float() * size).bfloat16()
+    close16(prefix_call(c), prefix64(c), 2e-3 * weighted_magnitude(c))
+
+
 def test_prefix_equals_whole_sequences():
     """The same keys as one block table per sequence, through paged_attention."""
     past, new, P, H, KV, d = [40, 7, 0], [1, 1, 1], 320, 32, 8, 128
