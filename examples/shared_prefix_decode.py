@@ -99,7 +99,7 @@ def serve(*, batch=64, prefix=4096, prompt=48, steps=32, hidden=2048, heads=16, 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        step()  # before the capture: scratch and status word
+        step()  # before the capture: the first call on a device allocates its status word
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=side):

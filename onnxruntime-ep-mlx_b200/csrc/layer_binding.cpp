@@ -13,8 +13,12 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <atomic>
 #include <map>
+#include <memory>
+#include <mutex>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "b200_layer.h"
@@ -149,15 +153,77 @@ int32_t* status_word(int device) {
   return static_cast<int32_t*>(it->second.data_ptr());
 }
 
-// Scratch per (device, stream), so calls on different streams never share it.  A buffer that became too
-// small is kept: a captured graph may still use it (sizes at least double, so the kept ones together stay
-// below the current one).
-std::vector<Tensor>& scratch(int device, cudaStream_t stream) {
-  static auto* kept = new std::map<std::pair<int, cudaStream_t>, std::vector<Tensor>>();  // until exit
-  return (*kept)[{device, stream}];
+// Captures whose graphs, and all that was instantiated from them, are gone.  Filled by the CUDA driver's
+// threads, which may not make CUDA calls then.
+struct Ended {
+  std::atomic<bool> any{false};
+  std::mutex mutex;
+  std::vector<unsigned long long> captures;
+};
+Ended& ended() {
+  static auto* e = new Ended;  // until exit
+  return *e;
 }
 
-// Run an operator with a workspace: the caller's, or the stream's own, grown where too small.
+// Scratch of a stream's eager calls, or of the calls that one capture took from a stream: either follow one
+// another, and calls that may overlap never share it.  A graph is replayed wherever and whenever its owner
+// likes, so each capture has buffers of its own.  They live as long as the graph and its instances; one that
+// became too small is kept, since earlier calls of the capture use it.
+struct Scratch {
+  bool captured = false;
+  std::vector<Tensor> buffers;  // the last one is the current one
+};
+using StreamScratch = std::map<std::pair<int, cudaStream_t>, Scratch>;
+
+void forget_ended(std::map<unsigned long long, StreamScratch>& captures) {
+  Ended& e = ended();
+  if (!e.any.load(std::memory_order_acquire)) return;
+  const std::lock_guard<std::mutex> lock(e.mutex);
+  for (const auto id : e.captures) captures.erase(id);
+  e.captures.clear();
+  e.any.store(false, std::memory_order_release);
+}
+
+// `id` joins the ended captures when its graph and the last instance are destroyed.
+void tell_end(unsigned long long id, cudaGraph_t graph) {
+  auto note = std::make_unique<unsigned long long>(id);
+  cudaUserObject_t object;
+  C10_CUDA_CHECK(cudaUserObjectCreate(
+      &object, note.get(),
+      [](void* p) {
+        const std::unique_ptr<unsigned long long> note(static_cast<unsigned long long*>(p));
+        try {
+          Ended& e = ended();
+          const std::lock_guard<std::mutex> lock(e.mutex);
+          e.captures.push_back(*note);
+          e.any.store(true, std::memory_order_release);
+        } catch (...) {  // the buffers stay until exit
+        }
+      },
+      1, cudaUserObjectNoDestructorSync));
+  note.release();
+  const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+  C10_CUDA_CHECK(e);
+}
+
+Scratch& scratch(int device, cudaStream_t stream) {
+  static auto* eager = new StreamScratch;  // both until exit
+  static auto* captures = new std::map<unsigned long long, StreamScratch>;
+  forget_ended(*captures);
+  cudaStreamCaptureStatus status;
+  C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &status));
+  if (status != cudaStreamCaptureStatusActive) return (*eager)[{device, stream}];
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo_v2(stream, &status, &id, &graph, nullptr, nullptr));
+  if (captures->find(id) == captures->end()) tell_end(id, graph);
+  Scratch& own = (*captures)[id][{device, stream}];
+  own.captured = true;
+  return own;
+}
+
+// Run an operator with a workspace: the caller's, or the stream's or capture's own, grown where too small.
 template <typename P>
 void run_with_workspace(const char* op, P* p, PyObject* workspace, int device, cudaStream_t stream,
                         int (*size)(const P*, size_t*), int (*run)(const P*, void*)) {
@@ -169,15 +235,17 @@ void run_with_workspace(const char* op, P* p, PyObject* workspace, int device, c
     p->workspace_bytes = w.numel();
     return checked(run(p, stream));
   }
-  auto& kept = scratch(device, stream);
-  p->workspace = kept.empty() ? nullptr : kept.back().data_ptr();
-  p->workspace_bytes = kept.empty() ? 0 : kept.back().numel();
+  Scratch& own = scratch(device, stream);
+  auto& buffers = own.buffers;
+  p->workspace = buffers.empty() ? nullptr : buffers.back().data_ptr();
+  p->workspace_bytes = buffers.empty() ? 0 : buffers.back().numel();
   const int code = run(p, stream);
   size_t need = 0;
   if (code != B200_ERR_WORKSPACE || size(p, &need) != B200_OK || need <= p->workspace_bytes) return checked(code);
-  kept.push_back(empty({(int64_t)std::max<size_t>({need, (size_t)1 << 20, 2 * p->workspace_bytes})}, at::kByte, device));
-  p->workspace = kept.back().data_ptr();
-  p->workspace_bytes = kept.back().numel();
+  if (!own.captured) buffers.clear();  // the allocator hands it to later work of this stream only
+  buffers.push_back(empty({(int64_t)std::max<size_t>({need, (size_t)1 << 20, 2 * p->workspace_bytes})}, at::kByte, device));
+  p->workspace = buffers.back().data_ptr();
+  p->workspace_bytes = buffers.back().numel();
   checked(run(p, stream));
 }
 

@@ -5,8 +5,10 @@ Torch only owns device memory and the current stream; the work runs in ``libb200
 through the native binding ``_layer``, which checks the tensors and allocates the outputs.  Argument
 errors raise ``B200Error``.  Errors that only the device can see (a slot, position, length or block id
 out of range) set a status word; ``check_status=True`` synchronises and raises them.  Every function
-takes ``stream=`` (default: the current stream).  The first call on a device, and the first on a
-stream, allocate their status word and scratch: make them before a graph capture.
+takes ``stream=`` (default: the current stream).  Scratch belongs to the stream of the calls; calls that
+are captured in a CUDA graph get scratch of that graph, which lives as long as the graph, so graphs may
+be replayed at the same time as each other and as other calls.  The first call on a device allocates its
+status word: make it before a graph capture.
 """
 
 from __future__ import annotations
@@ -86,8 +88,9 @@ def shared_prefix_attention(query, key_cache, value_cache, cumulative_sequence_l
 
     Every key is read from the caches (``[blocks, block_size, kv_num_heads, d]``, fp16 / bf16), the
     new tokens' included: append them first.  Metadata are int32 device tensors.  Returns the output
-    ``[tokens, num_heads * d]``.  The scratch is the current stream's own buffer unless ``workspace``
-    (uint8, at least ``b200_shared_prefix_attention_workspace_size`` bytes) is given.
+    ``[tokens, num_heads * d]``.  The scratch is the current stream's own buffer, or in a graph capture
+    the graph's, unless ``workspace`` (uint8, at least ``b200_shared_prefix_attention_workspace_size``
+    bytes) is given.
     """
     if stream is not None:
         return _on_stream(stream, shared_prefix_attention, query, key_cache, value_cache, cumulative_sequence_length,

@@ -754,6 +754,87 @@ def test_layer_in_a_graph():
     del graph
 
 
+def scratch_calls():
+    """Two callables that need scratch, of different sizes: a rotation with more tokens than are searched and an
+    attention call of four launches.  Each returns all that it wrote."""
+    calls = []
+    for seed, nt, prefix in ((5, 8500, ([300] * 40, [1] * 40, 3000, 32, 8, 128)), (6, 9000, ([5, 0, 90], [60, 1, 200], 1000, 16, 4, 64))):
+        rope, attention = rope_case(seed, nt, 4, 1, 64, 64), prefix_case(seed, *prefix)
+        rope["slots"][nt // 2:nt // 2 + 3000] = rope["slots"][:3000].clone()  # duplicates: the table decides
+
+        def call(rope=rope, attention=attention):
+            q, kc, vc = rope_call(rope, rope["kc"], rope["vc"], check_status=False)
+            return q, kc, vc, prefix_call(attention, check_status=False)
+
+        calls.append(call)
+    return calls
+
+
+def same(got, want):
+    return all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("on_side", [False, True])
+def test_captured_graphs_have_scratch_of_their_own(on_side):
+    """Two graphs captured on one stream (torch's default capture stream, or one that ran the calls before),
+    replayed on two streams at once and beside eager calls on a third and on the capture stream."""
+    calls = scratch_calls()
+    capture = torch.cuda.Stream() if on_side else None
+    wants = [[t.clone() for t in call()] for call in calls]
+    if on_side:
+        with torch.cuda.stream(capture):
+            for call in calls:
+                call()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=capture):
+            outs.append(call())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    eager = prefix_case(8, [50, 7] * 20, [1] * 40, 2000, 32, 8, 128)
+    want = prefix_call(eager)
+    for _ in range(10):
+        got = []
+        for _ in range(4):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            got.append(prefix_call(eager, check_status=False))
+            if on_side:
+                with torch.cuda.stream(capture):
+                    got.append(prefix_call(eager, check_status=False))
+        torch.cuda.synchronize()
+        assert same(outs[0], wants[0]) and same(outs[1], wants[1]) and all(torch.equal(g, want) for g in got)
+    del graphs, graph
+
+
+def test_scratch_of_a_graph_ends_with_it():
+    """Captured again and again, the calls hold no more memory than one graph's."""
+    import time
+
+    call = scratch_calls()[0]
+    call()
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        return torch.cuda.memory_allocated()
+
+    first = capture()
+    for _ in range(20):
+        call()
+        torch.cuda.synchronize()
+        if capture() <= first:  # the driver reports a graph's end from a thread of its own
+            break
+        time.sleep(0.1)
+    else:
+        pytest.fail("scratch of deleted graphs is not freed")
+
+
 def test_example_layer_against_whole_sequences():
     """The example's last decode step, recomputed from its caches with every sequence's keys in one piece."""
     import importlib.util
