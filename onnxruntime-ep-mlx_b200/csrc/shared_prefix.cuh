@@ -57,7 +57,7 @@ constexpr int kOwnTile = 16;  // keys per tile of the own kernel
 constexpr int kOwnWarps = 4;  // warps per CTA
 constexpr int kOwnCtasPerSm = 3;  // its shared memory, 65 KB per CTA, leaves room for three
 constexpr int kPrefixKeys = 128;  // keys per tile of the tensor-core kernel
-constexpr float kCopyScale = 2048.f;  // factor on the values of v_copy, taken out of the pass's results
+constexpr float kCopyScaleLog2 = 11.f, kCopyScale = 2048.f;  // factor on the values of v_copy, taken out of the pass's triples
 
 cudaError_t launch_shared_prefix_tc(const SharedPrefixArgs& a, const SharedPrefixMaps& maps, int num_sms,
                                     cudaStream_t stream);

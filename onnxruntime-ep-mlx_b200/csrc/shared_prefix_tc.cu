@@ -729,8 +729,8 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
       if (!wait_softmax(&bars.o_done[w], items++)) break;
       tc::fence_after_sync();
       const int64_t at = (int64_t)m.slab * a.rows + (int64_t)tok * H + m.kh * g + hl;
-      if (row_ok) a.slab_ml[at] = make_float2(m_run, l_run);
-      const float unscale = copied ? 1.f / kCopyScale : 1.f;
+      // values times 2^11 from the copy: (m, l, o) stands for 2^m l and 2^m o / 2^11, so 11 comes off m and l takes the factor
+      if (row_ok) a.slab_ml[at] = copied ? make_float2(m_run - kCopyScaleLog2, l_run * kCopyScale) : make_float2(m_run, l_run);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
@@ -739,8 +739,7 @@ __global__ void __launch_bounds__((TcLayout<D, BESIDE>::kBoundThreads), 1) share
         if (row_ok) {
           float4* dst = reinterpret_cast<float4*>(a.slab_o + at * D + c * 32);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(o[4 * i] * unscale, o[4 * i + 1] * unscale, o[4 * i + 2] * unscale, o[4 * i + 3] * unscale);
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
       tc::fence_before_sync();
