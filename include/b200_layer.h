@@ -110,7 +110,8 @@ typedef struct B200RotaryAppendParams {
   const int32_t* slot_mapping; /* [num_tokens]                                                  */
   const float* k_scale;        /* fp8 caches: [num_blocks, kv_num_heads]                        */
   const float* v_scale;
-  void* workspace;             /* >= b200_rotary_append_workspace_size(); NULL when that is 0   */
+  void* workspace;             /* >= b200_rotary_append_workspace_size() bytes, aligned to 4;
+                                  NULL when that is 0                                           */
   size_t workspace_bytes;
   int32_t* device_status;      /* see b200_layer_read_status; NULL = not reported               */
 } B200RotaryAppendParams;
@@ -165,7 +166,8 @@ typedef struct B200SharedPrefixParams {
   const int32_t* prefix_block_table;         /* [prefix_blocks]; may be NULL without a prefix   */
   const void* head_sink;       /* [num_heads] in T or NULL                                      */
   void* output;                /* [num_tokens, num_heads * head_size]                           */
-  void* workspace;             /* >= b200_shared_prefix_attention_workspace_size()              */
+  void* workspace;             /* >= b200_shared_prefix_attention_workspace_size() bytes,
+                                  aligned to 16                                                 */
   size_t workspace_bytes;
   int32_t* device_status;      /* see b200_layer_read_status; NULL = not reported               */
 } B200SharedPrefixParams;

@@ -52,6 +52,16 @@ int guarded(const char* op, F&& body) {
 
 int64_t dense(int64_t stride, int64_t width) { return stride ? stride : width; }
 
+// B200_OK for a workspace of at least `need` bytes whose address is a multiple of `align`.
+int check_workspace(const char* op, const char* size_call, const void* workspace, size_t bytes, size_t need, size_t align) {
+  if (!need) return B200_OK;
+  if (!workspace || bytes < need)
+    return set_error(B200_ERR_WORKSPACE, std::string(op) + ": workspace missing or smaller than " + size_call + "()");
+  if (reinterpret_cast<uintptr_t>(workspace) % align)
+    return set_error(B200_ERR_WORKSPACE, std::string(op) + ": workspace must be aligned to " + std::to_string(align) + " bytes");
+  return B200_OK;
+}
+
 // ---- skip RMS norm
 constexpr const char* kNorm = "SkipRmsNorm";
 
@@ -207,9 +217,8 @@ int b200_rotary_append(const B200RotaryAppendParams* params, void* stream) {
     if (int rc = check_rope(&p)) return rc;
     if (p.num_tokens == 0) return B200_OK;
     const size_t need = b200::rotary_append_workspace(p);
-    if (need && (!p.workspace || p.workspace_bytes < need))
-      return set_error(B200_ERR_WORKSPACE,
-                       "RotaryAppend: workspace missing or smaller than b200_rotary_append_workspace_size()");
+    if (int rc = check_workspace(kRope, "b200_rotary_append_workspace_size", p.workspace, p.workspace_bytes, need, sizeof(int)))
+      return rc;
     return launched(kRope, b200::launch_rotary_append(p, sm_count(0), static_cast<cudaStream_t>(stream)));
   });
 }
@@ -230,9 +239,9 @@ int b200_shared_prefix_attention(const B200SharedPrefixParams* params, void* str
     if (p.num_tokens == 0) return B200_OK;
     const int sms = sm_count(p.num_sms);
     const size_t need = b200::shared_prefix_workspace(p, sms);
-    if (need && (!p.workspace || p.workspace_bytes < need))
-      return set_error(B200_ERR_WORKSPACE, "SharedPrefixAttention: workspace missing or smaller than "
-                                           "b200_shared_prefix_attention_workspace_size()");
+    if (int rc = check_workspace(kPrefix, "b200_shared_prefix_attention_workspace_size", p.workspace, p.workspace_bytes,
+                                 need, 16))  // 16-byte accesses and a TMA source
+      return rc;
     return launched(kPrefix, b200::launch_shared_prefix(p, sms, static_cast<cudaStream_t>(stream)));
   });
 }

@@ -90,7 +90,7 @@ def shared_prefix_attention(query, key_cache, value_cache, cumulative_sequence_l
     new tokens' included: append them first.  Metadata are int32 device tensors.  Returns the output
     ``[tokens, num_heads * d]``.  The scratch is the current stream's own buffer, or in a graph capture
     the graph's, unless ``workspace`` (uint8, at least ``b200_shared_prefix_attention_workspace_size``
-    bytes) is given.
+    bytes, aligned to 16) is given.
     """
     if stream is not None:
         return _on_stream(stream, shared_prefix_attention, query, key_cache, value_cache, cumulative_sequence_length,

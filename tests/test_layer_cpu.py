@@ -146,3 +146,18 @@ def test_empty_calls_touch_nothing():
     a = prefix()
     a.num_tokens, a.query = 0, None
     assert LIB.b200_shared_prefix_attention(ctypes.byref(a), None) == _capi.B200_OK
+
+
+@pytest.mark.parametrize("make,name,change,align", [(rope, "rotary_append", dict(num_tokens=8193), 4),
+                                                    (prefix, "shared_prefix_attention", {}, 16)])
+def test_misaligned_workspaces_are_refused(make, name, change, align):
+    p = make()
+    for field, value in change.items():
+        setattr(p, field, value)
+    n = ctypes.c_size_t(0)
+    assert getattr(LIB, f"b200_{name}_workspace_size")(ctypes.byref(p), ctypes.byref(n)) == _capi.B200_OK and n.value
+    p.workspace_bytes = n.value + 64
+    for off in {1, 2, align // 2, align - 1, align + 1}:
+        p.workspace = 0x100000 + off
+        assert getattr(LIB, f"b200_{name}")(ctypes.byref(p), None) == WORKSPACE
+        assert f"aligned to {align} bytes" in LIB.b200_last_error().decode()
