@@ -7,7 +7,8 @@
  *   b200_shared_prefix_attention  causal attention over paged caches for a batch whose sequences
  *                                 share one prefix; the prefix is attended once for all of them
  *
- * The conventions are those of b200_paged.h: device pointers on the current device, `stream` a
+ * The conventions are those of b200_paged.h: device pointers on the current device (each aligned to
+ * its elements, workspaces as stated there; anything else is refused), `stream` a
  * cudaStream_t as void*, a B200_* status code as the result, the message in b200_last_error(),
  * no exception leaves the library.  The calls are asynchronous and allocate nothing; they can be
  * captured in a CUDA graph.

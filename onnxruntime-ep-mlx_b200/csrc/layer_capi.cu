@@ -2,6 +2,7 @@
 // status word.  Every check runs before anything touches the device.
 #include <cmath>
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 #include "b200_kernels.h"
@@ -52,6 +53,13 @@ int guarded(const char* op, F&& body) {
 
 int64_t dense(int64_t stride, int64_t width) { return stride ? stride : width; }
 
+// Whether every address (NULL passes) is a multiple of its element's size.
+bool aligned(std::initializer_list<const void*> addresses, size_t size) {
+  uintptr_t bits = 0;
+  for (const void* a : addresses) bits |= reinterpret_cast<uintptr_t>(a);
+  return bits % size == 0;
+}
+
 // B200_OK for a workspace of at least `need` bytes whose address is a multiple of `align`.
 int check_workspace(const char* op, const char* size_call, const void* workspace, size_t bytes, size_t need, size_t align) {
   if (!need) return B200_OK;
@@ -90,6 +98,8 @@ int check_norm(B200SkipRmsNormParams* p) {
   if (fp8 && (p->out == p->x || p->out == p->residual || p->out == p->residual_out))
     return invalid(kNorm, "an fp8 output cannot share a 16-bit tensor's memory");
   if (p->out == p->residual_out) return invalid(kNorm, "out and residual_out must differ");
+  if (!aligned({p->x, p->residual, p->weight, p->residual_out, fp8 ? nullptr : p->out}, 2) || !aligned({p->scales}, 4))
+    return invalid(kNorm, "a tensor is not aligned to its elements");
   return B200_OK;
 }
 
@@ -139,6 +149,11 @@ int check_rope(B200RotaryAppendParams* p) {
       !p->cos_cache || !p->sin_cache || !p->slot_mapping)
     return invalid(kRope, "missing required tensor");
   if (fp8 && (!p->k_scale || !p->v_scale)) return invalid(kRope, "fp8 caches require k_scale and v_scale");
+  if (!aligned({p->query, p->key, p->value, p->output}, 2) || !aligned({p->key_cache, p->value_cache}, fp8 ? 1 : 2) ||
+      !aligned({p->cos_cache, p->sin_cache}, p->table_dtype == B200_DTYPE_FLOAT ? 4 : 2) ||
+      !aligned({p->position_ids}, p->position_dtype == B200_DTYPE_INT64 ? 8 : 4) ||
+      !aligned({p->slot_mapping, p->k_scale, p->v_scale, p->device_status}, 4))
+    return invalid(kRope, "a tensor is not aligned to its elements");
   return B200_OK;
 }
 
@@ -176,6 +191,9 @@ int check_prefix(B200SharedPrefixParams* p) {
   if (!p->query || !p->key_cache || !p->value_cache || !p->output || !p->cumulative_sequence_length ||
       !p->past_seqlens || !p->block_table || (p->prefix_length > 0 && !p->prefix_block_table))
     return invalid(kPrefix, "missing required tensor");
+  if (!aligned({p->query, p->key_cache, p->value_cache, p->head_sink, p->output}, 2) ||
+      !aligned({p->cumulative_sequence_length, p->past_seqlens, p->block_table, p->prefix_block_table, p->device_status}, 4))
+    return invalid(kPrefix, "a tensor is not aligned to its elements");
   if (p->scale == 0.f) p->scale = 1.0f / std::sqrt((float)p->head_size);
   return B200_OK;
 }
@@ -247,7 +265,8 @@ int b200_shared_prefix_attention(const B200SharedPrefixParams* params, void* str
 }
 
 int b200_layer_read_status(int32_t* device_status, void* stream_ptr) {
-  if (!device_status) return set_error(B200_ERR_INVALID_ARGUMENT, "layer status: no status word");
+  if (!device_status || !aligned({device_status}, 4))
+    return set_error(B200_ERR_INVALID_ARGUMENT, "layer status: no status word, or a misaligned one");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   int bits = 0;
   cudaError_t e = cudaMemcpyAsync(&bits, device_status, sizeof(int), cudaMemcpyDeviceToHost, stream);

@@ -161,3 +161,26 @@ def test_misaligned_workspaces_are_refused(make, name, change, align):
         p.workspace = 0x100000 + off
         assert getattr(LIB, f"b200_{name}")(ctypes.byref(p), None) == WORKSPACE
         assert f"aligned to {align} bytes" in LIB.b200_last_error().decode()
+
+
+@pytest.mark.parametrize("make,entry,change,fields", [
+    (norm, "b200_skip_rms_norm", {}, dict(x=1, residual=1, weight=1, out=1, residual_out=1)),
+    (norm, "b200_skip_rms_norm", dict(out_dtype=E4M3), dict(x=1, scales=2)),
+    (rope, "b200_rotary_append", dict(table_dtype=FP32),
+     dict(query=1, key=1, value=1, output=1, key_cache=1, value_cache=1, cos_cache=2, sin_cache=2, position_ids=4,
+          slot_mapping=2, device_status=2)),
+    (rope, "b200_rotary_append", dict(cache_dtype=E4M3, k_scale=0x20000, v_scale=0x21000, position_dtype=_capi.DTYPE_INT32),
+     dict(cos_cache=1, sin_cache=1, position_ids=2, k_scale=2, v_scale=2)),
+    (prefix, "b200_shared_prefix_attention", {},
+     dict(query=1, key_cache=1, value_cache=1, head_sink=1, output=1, cumulative_sequence_length=2, past_seqlens=2,
+          block_table=2, prefix_block_table=2, device_status=2)),
+])
+def test_misaligned_tensors_are_refused(make, entry, change, fields):
+    for field, off in fields.items():
+        p = make()
+        for name, value in change.items():
+            setattr(p, name, value)
+        setattr(p, field, (getattr(p, field) or 0x30000) + off)
+        assert getattr(LIB, entry)(ctypes.byref(p), None) == INVALID, field
+        assert "not aligned to its elements" in LIB.b200_last_error().decode()
+    assert LIB.b200_layer_read_status(0x30002, None) == INVALID
