@@ -155,7 +155,7 @@ typedef struct B200SharedPrefixParams {
   int32_t max_blocks_per_seq;  /* columns of block_table                                        */
   int32_t prefix_length;       /* keys of the prefix, >= 0                                      */
   int32_t prefix_blocks;       /* entries of prefix_block_table                                 */
-  int32_t num_sms;             /* 0 = query the device                                          */
+  int32_t num_sms;             /* 0 = query the device; at most 1024                            */
   int64_t query_row_stride;    /* elements between tokens; 0 = num_heads * head_size            */
   int64_t output_row_stride;
   const void* query;           /* [num_tokens, num_heads * head_size]                           */

@@ -159,6 +159,7 @@ int check_rope(B200RotaryAppendParams* p) {
 
 // ---- shared prefix attention
 constexpr const char* kPrefix = "SharedPrefixAttention";
+constexpr int kMaxSms = 1024;
 
 int check_prefix_shapes(B200SharedPrefixParams* p) {
   if (p->num_heads <= 0 || p->kv_num_heads <= 0 || p->num_heads % p->kv_num_heads != 0)
@@ -176,6 +177,8 @@ int check_prefix_shapes(B200SharedPrefixParams* p) {
     return invalid(kPrefix, "prefix_length exceeds prefix_block_table");
   if ((int64_t)p->prefix_length + (int64_t)p->max_blocks_per_seq * p->block_size > INT32_MAX)
     return unsupported(kPrefix, "a sequence's keys exceed int32");
+  // grids and the workspace are counted from it in 32 bits
+  if (p->num_sms > kMaxSms) return invalid(kPrefix, "num_sms exceeds " + std::to_string(kMaxSms));
   return B200_OK;
 }
 

@@ -184,3 +184,14 @@ def test_misaligned_tensors_are_refused(make, entry, change, fields):
         assert getattr(LIB, entry)(ctypes.byref(p), None) == INVALID, field
         assert "not aligned to its elements" in LIB.b200_last_error().decode()
     assert LIB.b200_layer_read_status(0x30002, None) == INVALID
+
+
+@pytest.mark.parametrize("num_sms", [1025, 200_000_000, 2 ** 31 - 1])
+def test_num_sms_is_bounded(num_sms):
+    p, n = prefix(), ctypes.c_size_t(0)
+    p.num_sms, p.workspace, p.workspace_bytes = num_sms, 0x100000, 1 << 62
+    assert LIB.b200_shared_prefix_attention(ctypes.byref(p), None) == INVALID
+    assert "num_sms" in LIB.b200_last_error().decode()
+    assert LIB.b200_shared_prefix_attention_workspace_size(ctypes.byref(p), ctypes.byref(n)) == INVALID
+    p.num_sms = 1024
+    assert LIB.b200_shared_prefix_attention_workspace_size(ctypes.byref(p), ctypes.byref(n)) == _capi.B200_OK and n.value < 1 << 40
