@@ -183,9 +183,10 @@ B200_API int b200_shared_prefix_attention(const B200SharedPrefixParams* p, void*
 
 /* ---- status ------------------------------------------------------------------------------ */
 
-/* Synchronise `stream`, read and clear a status word that calls of this header were given as
- * device_status (zero it once before its first use; the calls only set bits).  B200_ERR_FAIL for
- * invalid metadata, B200_ERR_DEVICE for a device wait that ran out. */
+/* Synchronise `stream`, read a status word that calls of this header were given as device_status (zero
+ * it once before its first use; the calls only set bits) and clear the bits that it held.  B200_ERR_FAIL
+ * for invalid metadata, B200_ERR_DEVICE for a device wait that ran out.  A report does not say which call
+ * made it: give streams, and graphs that are replayed elsewhere, a word each. */
 B200_API int b200_layer_read_status(int32_t* device_status, void* stream);
 
 /* sizeof of the parameter structs (0 skip RMS norm, 1 rotary append, 2 shared prefix), for binding

@@ -140,17 +140,34 @@ Tensor empty(at::IntArrayRef shape, ScalarType type, int device) {
   return at::detail::empty_cuda(shape, type, c10::Device(c10::kCUDA, (c10::DeviceIndex)device), std::nullopt);
 }
 
-// One status word per device, zeroed once: calls only set bits, b200_layer_read_status clears them.
-int32_t* status_word(int device) {
-  static auto* words = new std::map<int, Tensor>();  // kept until exit
-  auto it = words->find(device);
-  if (it == words->end()) {
-    Tensor word = empty({1}, at::kInt, device);
-    word.zero_();
-    C10_CUDA_CHECK(cudaDeviceSynchronize());  // zeroed before any stream uses it
-    it = words->emplace(device, std::move(word)).first;
+// Status word per (device, stream), zeroed once: calls only set bits, b200_layer_read_status clears them.
+// Calls on different streams never share one, so a call's report goes to nobody else; a captured call reports
+// to the stream that it was captured on.  Words come in blocks, so that a capture on a stream without a word
+// gets one without an allocation.
+constexpr int kBlockWords = 1024;
+using StreamWords = std::map<std::pair<int, cudaStream_t>, int32_t*>;
+StreamWords& stream_words() {
+  static auto* words = new StreamWords;  // until exit, like the blocks below
+  return *words;
+}
+int32_t* status_word(const char* op, int device, cudaStream_t stream) {
+  static auto* blocks = new std::map<int, std::pair<std::vector<Tensor>, int>>;  // device -> blocks, words used
+  StreamWords& words = stream_words();
+  const auto it = words.find({device, stream});
+  if (it != words.end()) return it->second;
+  auto& [kept, used] = (*blocks)[device];
+  if (used == (int)kept.size() * kBlockWords) {
+    cudaStreamCaptureStatus status;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &status));
+    if (status != cudaStreamCaptureStatusNone) bad(op, "the first call on a device cannot be captured: make one before");
+    Tensor block = empty({kBlockWords}, at::kInt, device);
+    block.zero_();
+    C10_CUDA_CHECK(cudaStreamSynchronize(stream));  // zeroed before any other stream uses it
+    kept.push_back(std::move(block));
   }
-  return static_cast<int32_t*>(it->second.data_ptr());
+  int32_t* word = static_cast<int32_t*>(kept.back().data_ptr()) + used % kBlockWords;
+  ++used;
+  return words[{device, stream}] = word;
 }
 
 // Captures whose graphs, and all that was instantiated from them, are gone.  Filled by the CUDA driver's
@@ -427,8 +444,8 @@ PyObject* rotary_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
       p.output_row_stride = rows(op, "output", o, nt, H * d, type, device);
       p.output = o.data_ptr();
     }
-    p.device_status = status_word(device);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    p.device_status = status_word(op, device, stream);
     if (nt <= B200_ROTARY_APPEND_SCAN_TOKENS) checked(b200_rotary_append(&p, stream));
     else run_with_workspace(op, &p, args[17], device, stream, b200_rotary_append_workspace_size, b200_rotary_append);
     return tuple_of({given_or(args[16], std::move(out)), shared(args[3]), shared(args[4])});
@@ -490,19 +507,22 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n
       p.output_row_stride = rows(op, "output", o, nt, H * d, type, device);
       p.output = o.data_ptr();
     }
-    p.device_status = status_word(device);
-    run_with_workspace(op, &p, args[14], device, c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(),
-                       b200_shared_prefix_attention_workspace_size, b200_shared_prefix_attention);
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    p.device_status = status_word(op, device, stream);
+    run_with_workspace(op, &p, args[14], device, stream, b200_shared_prefix_attention_workspace_size,
+                       b200_shared_prefix_attention);
     return given_or(args[13], std::move(out));
   });
 }
 
-// device index -> None; raises what the calls so far reported on the current stream
+// device index -> None; raises what the current stream's calls on it reported since the last time
 PyObject* read_status(PyObject*, PyObject* arg) {
   return guarded([&]() -> PyObject* {
-    const int device = device_of("layer status", tensor("layer status", "tensor", arg));
+    const int device = integer("layer status", "device", arg);
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
-    checked(b200_layer_read_status(status_word(device), c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream()));
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    const auto it = stream_words().find({device, stream});
+    if (it != stream_words().end()) checked(b200_layer_read_status(it->second, stream));
     Py_RETURN_NONE;
   });
 }

@@ -201,6 +201,9 @@ int check_prefix(B200SharedPrefixParams* p) {
   return B200_OK;
 }
 
+// Clears what was read and nothing that was set since.
+__global__ void clear_bits_kernel(int32_t* status, int bits) { atomicAnd(status, ~bits); }
+
 }  // namespace
 
 extern "C" {
@@ -273,10 +276,12 @@ int b200_layer_read_status(int32_t* device_status, void* stream_ptr) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   int bits = 0;
   cudaError_t e = cudaMemcpyAsync(&bits, device_status, sizeof(int), cudaMemcpyDeviceToHost, stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(device_status, 0, sizeof(int), stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
   if (e != cudaSuccess) return launched("layer status", e);
   if (bits == 0) return B200_OK;
+  clear_bits_kernel<<<1, 1, 0, stream>>>(device_status, bits);
+  b200::add_launches(1);
+  if ((e = cudaGetLastError()) != cudaSuccess) return launched("layer status", e);
   if (bits & (b200::kStatusBadCumulative | b200::kStatusBadPast | b200::kStatusBadCapacity))
     return set_error(B200_ERR_FAIL, "SharedPrefixAttention: inconsistent cumulative lengths, past lengths or block table");
   if (bits & b200::kStatusBadBlock)

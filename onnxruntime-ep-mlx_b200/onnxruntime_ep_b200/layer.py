@@ -4,7 +4,9 @@
 Torch only owns device memory and the current stream; the work runs in ``libb200_paged.so``, called
 through the native binding ``_layer``, which checks the tensors and allocates the outputs.  Argument
 errors raise ``B200Error``.  Errors that only the device can see (a slot, position, length or block id
-out of range) set a status word; ``check_status=True`` synchronises and raises them.  Every function
+out of range) set the status word of the stream; ``check_status=True`` synchronises and raises what the
+stream's calls have reported, as does ``check_status(stream)``.  A captured call reports to the stream that
+it was captured on.  Every function
 takes ``stream=`` (default: the current stream).  Scratch belongs to the stream of the calls; calls that
 are captured in a CUDA graph get scratch of that graph, which lives as long as the graph, so graphs may
 be replayed at the same time as each other and as other calls.  The first call on a device allocates its
@@ -33,6 +35,15 @@ def _on_stream(stream, fn, *args, **kwargs):
     """``fn`` with ``stream`` current, so what it allocates belongs to the stream that uses it."""
     with torch.cuda.stream(stream):
         return fn(*args, **kwargs)
+
+
+def check_status(stream=None):
+    """Synchronise ``stream`` (default: the current one) and raise what its calls have reported since the last
+    check.  For the calls in a CUDA graph, ``stream`` is the one they were captured on: wait for the replays
+    first, then check it."""
+    stream = stream if stream is not None else torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        _layer.read_status(stream.device.index)
 
 
 def skip_rms_norm(x, residual, weight, *, epsilon=1e-6, out_dtype=None, group_size=0, output=None, scales=None,
@@ -75,7 +86,7 @@ def rotary_append(query, key, value, key_cache, value_cache, position_ids, cos_c
                                   slot_mapping, num_heads, kv_num_heads, axis_sections, rotary_interleaved, rotary_offset,
                                   k_scale, v_scale, output, workspace)
     if check_status:
-        _layer.read_status(query)
+        _layer.read_status(query.get_device())
     return result
 
 
@@ -101,5 +112,5 @@ def shared_prefix_attention(query, key_cache, value_cache, cumulative_sequence_l
                                             block_table, prefix_block_table, prefix_length, num_heads, kv_num_heads, scale,
                                             softcap, head_sink, output, workspace, num_sms)
     if check_status:
-        _layer.read_status(query)
+        _layer.read_status(query.get_device())
     return result

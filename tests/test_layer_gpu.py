@@ -20,7 +20,7 @@ if not torch.cuda.is_available():
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
 from onnxruntime_ep_b200 import (B200Error, kv_append, paged_attention, rotary_append, shared_prefix_attention,  # noqa: E402
-                                 skip_rms_norm)
+                                 layer, skip_rms_norm)
 from oracle import tolerance  # noqa: E402
 
 FP8 = torch.float8_e4m3fn
@@ -807,6 +807,50 @@ def test_captured_graphs_have_scratch_of_their_own(on_side):
         torch.cuda.synchronize()
         assert same(outs[0], wants[0]) and same(outs[1], wants[1]) and all(torch.equal(g, want) for g in got)
     del graphs, graph
+
+
+def bad_slots(c):
+    return {**c, "slots": c["slots"].clone().fill_(1 << 30)}
+
+
+def test_status_belongs_to_the_stream_of_the_call():
+    """A bad call on one stream is not another stream's error, and stays its own stream's until read."""
+    c, a = rope_case(3, 20, 4, 2, 64, 64), prefix_case(6, [20, 40], [1, 1], 100, 8, 2, 64)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    rope_call(bad_slots(c), c["kc"], c["vc"], check_status=False, stream=one)
+    torch.cuda.synchronize()
+    rope_call(c, c["kc"], c["vc"], stream=two)
+    prefix_call(a, stream=two)
+    prefix_call(a)
+    layer.check_status(two)
+    with pytest.raises(B200Error, match="slot_mapping"):
+        prefix_call(a, stream=one)
+    layer.check_status(one)  # read once
+    rope_call(bad_slots(c), c["kc"], c["vc"], check_status=False, stream=one)
+    with pytest.raises(B200Error, match="slot_mapping"):
+        layer.check_status(one)
+
+
+def test_status_of_a_graph_is_on_its_capture_stream():
+    c = rope_case(3, 20, 4, 2, 64, 64)
+    rope_call(c, c["kc"], c["vc"])  # the device's words exist
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    c["slots"] = c["slots"].clone()
+    with torch.cuda.graph(graph, stream=side):
+        rope_call(c, c["kc"], c["vc"], check_status=False)
+    graph.replay()
+    torch.cuda.synchronize()
+    layer.check_status(side)
+    c["slots"].fill_(-2)
+    graph.replay()
+    torch.cuda.synchronize()
+    good = rope_case(4, 20, 4, 2, 64, 64)
+    rope_call(good, good["kc"], good["vc"])
+    with pytest.raises(B200Error, match="slot_mapping"):
+        layer.check_status(side)
+    layer.check_status(side)
+    del graph
 
 
 def test_scratch_of_a_graph_ends_with_it():
