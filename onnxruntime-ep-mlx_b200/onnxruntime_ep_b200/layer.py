@@ -15,18 +15,30 @@ status word: make it before a graph capture.
 
 from __future__ import annotations
 
+import importlib
+
 import torch
 
 from . import _capi
 from ._capi import B200Error
 
-try:
-    from . import _layer
-except ImportError as e:
-    raise ImportError(f"onnxruntime_ep_b200/_layer.so cannot be loaded ({e}): build it with "
-                      "`make -C onnxruntime-ep-mlx_b200/csrc`") from e
 
-_layer.set_error_class(B200Error)
+class _Binding:
+    """The native module ``_layer``, loaded at the first use: it is built against one torch, and the rest of
+    the package needs neither it nor that torch."""
+
+    def __getattr__(self, name):
+        try:
+            module = importlib.import_module("._layer", __package__)
+        except ImportError as e:
+            raise ImportError(f"onnxruntime_ep_b200/_layer.so cannot be loaded ({e}): build it against this torch with "
+                              "`make -C onnxruntime-ep-mlx_b200/csrc`") from e
+        module.set_error_class(B200Error)
+        globals()["_layer"] = module
+        return getattr(module, name)
+
+
+_layer = _Binding()
 
 _FP8 = torch.float8_e4m3fn
 
