@@ -150,7 +150,7 @@ typedef struct B200SharedPrefixParams {
   float softcap;               /* 0 = none                                                      */
   int32_t act_dtype;           /* T of query, caches, head_sink, output: FLOAT16 or BFLOAT16    */
   int32_t num_tokens;          /* packed new tokens                                             */
-  int32_t batch;
+  int32_t batch;               /* positive, or 0 without tokens                                 */
   int32_t num_blocks, block_size;
   int32_t max_blocks_per_seq;  /* columns of block_table                                        */
   int32_t prefix_length;       /* keys of the prefix, >= 0                                      */

@@ -170,7 +170,7 @@ int check_prefix_shapes(B200SharedPrefixParams* p) {
   if (!is_act(p->act_dtype)) return invalid(kPrefix, "query and caches must be fp16 or bf16");
   if (p->num_blocks <= 0 || p->block_size <= 0) return invalid(kPrefix, "caches require positive block geometry");
   if ((int64_t)p->num_blocks * p->block_size > INT32_MAX) return unsupported(kPrefix, "cache slot count exceeds int32");
-  if (p->num_tokens < 0 || p->batch < 1 || p->max_blocks_per_seq < 0)
+  if (p->num_tokens < 0 || p->batch < (p->num_tokens > 0) || p->max_blocks_per_seq < 0)
     return invalid(kPrefix, "batch must be positive, num_tokens and max_blocks_per_seq not negative");
   if (p->prefix_length < 0 || p->prefix_blocks < 0 ||
       p->prefix_length > (int64_t)p->prefix_blocks * p->block_size)

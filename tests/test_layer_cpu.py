@@ -195,3 +195,15 @@ def test_num_sms_is_bounded(num_sms):
     assert LIB.b200_shared_prefix_attention_workspace_size(ctypes.byref(p), ctypes.byref(n)) == INVALID
     p.num_sms = 1024
     assert LIB.b200_shared_prefix_attention_workspace_size(ctypes.byref(p), ctypes.byref(n)) == _capi.B200_OK and n.value < 1 << 40
+
+
+def test_an_empty_batch_is_an_empty_call():
+    p, n = prefix(), ctypes.c_size_t(7)
+    p.num_tokens, p.batch = 0, 0
+    for field in ("query", "output", "cumulative_sequence_length", "past_seqlens", "block_table"):
+        setattr(p, field, None)
+    assert LIB.b200_shared_prefix_attention(ctypes.byref(p), None) == _capi.B200_OK
+    assert LIB.b200_shared_prefix_attention_workspace_size(ctypes.byref(p), ctypes.byref(n)) == _capi.B200_OK and n.value == 0
+    for batch, tokens in ((0, 1), (-1, 0)):
+        p.batch, p.num_tokens = batch, tokens
+        assert LIB.b200_shared_prefix_attention(ctypes.byref(p), None) == INVALID

@@ -719,6 +719,20 @@ def test_prefix_refusals():
         prefix_call(big, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
 
 
+def test_empty_calls():
+    """No rows, no tokens, no sequences."""
+    x = torch.empty(0, 256, device="cuda", dtype=torch.bfloat16)
+    codes, scales, res = skip_rms_norm(x, x, torch.ones(256, device="cuda", dtype=torch.bfloat16), out_dtype=FP8, group_size=64)
+    assert codes.shape == res.shape == (0, 256) and scales.shape == (0, 4)
+    c = rope_case(1, 4, 4, 2, 64, 64)
+    empty = {**c, "slots": c["slots"][:0], "pos": c["pos"][:, :0], **{n: c[n][:0] for n in "qkv"}}
+    assert rope_call(empty, c["kc"], c["vc"])[0].shape == (0, 256)
+    a = prefix_case(6, [20], [1], 100, 8, 2, 64)
+    none = {**a, "q": a["q"][:0], "cum": a["cum"][:1], "past": a["past"][:0], "table": a["table"][:0]}
+    assert prefix_call(none).shape == (0, 512)
+    assert prefix_call({**a, "q": a["q"][:0], "cum": a["cum"] * 0}).shape == (0, 512)
+
+
 def test_layer_in_a_graph():
     """The three operators captured in one CUDA graph and replayed on new inputs."""
     H, KV, d, B, P = 8, 2, 128, 5, 200
