@@ -176,27 +176,44 @@ __device__ __forceinline__ void copy_prefix_values(const SharedPrefixArgs& a) {
   __shared__ unsigned long long inexact_heads;
   if (threadIdx.x == 0) inexact_heads = 0;
   __syncthreads();
-  unsigned long long inexact = 0;
-#pragma unroll 4
-  for (int64_t i = (int64_t)(blockIdx.x - 1) * kPlanThreads + threadIdx.x; i < n; i += step) {
+  auto load = [&](int64_t i) {
     const int64_t key = i / vecs;
     const int32_t blk = __ldg(p.prefix_block_table + key / p.block_size);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (blk >= 0 && blk < p.num_blocks)  // the tensor-core kernel reports the others
-      v = __ldg(static_cast<const uint4*>(p.value_cache) + ((int64_t)blk * p.block_size + key % p.block_size) * vecs + (i - key * vecs));
+    if (blk < 0 || blk >= p.num_blocks) return make_uint4(0, 0, 0, 0);  // the tensor-core kernel reports these
+    return __ldg(static_cast<const uint4*>(p.value_cache) + ((int64_t)blk * p.block_size + key % p.block_size) * vecs + (i - key * vecs));
+  };
+  // bits 15 and 31: a magnitude of 0x4200 (32) and above, or below 0x3180 (2^-28) and not zero
+  auto outside_of = [](const uint4& v) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t o[4], outside = 0;
+    uint32_t outside = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      // bits 15 and 31: a magnitude of 0x4200 (32) and above, or below 0x3180 (2^-28) and not zero
       const uint32_t m = w[k] & 0x7fff7fffu;
-      outside |= (m + 0x3e003e00u) | (~((m | 0x80008000u) - 0x31803180u) & (m + 0x7fff7fffu));
-      const __half2 h = __floats2half2_rn(__uint_as_float(w[k] << 16) * kCopyScale, __uint_as_float(w[k] & 0xffff0000u) * kCopyScale);
+      outside |= (m + 0x3e003e00u) | (~((w[k] | 0x80008000u) - 0x31803180u) & (m + 0x7fff7fffu));
+    }
+    return outside & 0x80008000u;
+  };
+  const __nv_bfloat162 factor = __float2bfloat162_rn(kCopyScale);
+  const int64_t first = (int64_t)(blockIdx.x - 1) * kPlanThreads + threadIdx.x;
+  uint32_t outside = 0;
+#pragma unroll 4
+  for (int64_t i = first; i < n; i += step) {
+    const uint4 v = load(i);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
+    outside |= outside_of(v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]), factor);
+      const __half2 h = __float22half2_rn(__bfloat1622float2(x));
       o[k] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    if (outside & 0x80008000u) inexact |= 1ull << ((uint32_t)(i - key * vecs) / (uint32_t)(p.head_size / 8) & 63u);
     reinterpret_cast<uint4*>(a.v_copy)[i] = make_uint4(o[0], o[1], o[2], o[3]);
   }
+  unsigned long long inexact = 0;
+  if (outside)  // rare: which heads (named in the loop above, a call with 8192 keys took 1 us longer)
+    for (int64_t i = first; i < n; i += step)
+      if (outside_of(load(i))) inexact |= 1ull << ((uint32_t)(i % vecs) / (uint32_t)(p.head_size / 8) & 63u);
   if (inexact) atomicOr(&inexact_heads, inexact);
   __syncthreads();
   if (threadIdx.x == 0) a.v_inexact[blockIdx.x - 1] = inexact_heads;
@@ -258,8 +275,9 @@ __global__ void __launch_bounds__(kPlanThreads) shared_prefix_plan_kernel(const 
 // ---------------------------------------------------------------------------------------------
 // Merge: D / 4 lanes per (token, head) row join the row's triples, BATCH of them in flight.  Bound by the
 // slabs' reads, which come from L2 as far as the own keys' stream has left them there, and by the issue of
-// instructions: batches of 4 where a row has few triples (whole calls with 4 and 8: 4000 tokens and at most
-// 3 ranges 214 against 218 us, 256 tokens 335 against 338; 128 tokens and 9 ranges 89.7 against 89.0).
+// instructions: batches of 4 where a row has few triples (whole calls with 4 and 8, medians of four runs in turn: 256
+// tokens and at most 3 ranges 362 against 364 us; 31 sequences of drafted tokens 60 against 58, 128 tokens and 9 ranges
+// 98.2 against 97.8).
 // ---------------------------------------------------------------------------------------------
 constexpr int kMergeThreads = 128;
 constexpr int kFewRanges = 3;
@@ -414,8 +432,9 @@ size_t layout(const B200SharedPrefixParams& p, int num_sms, SharedPrefixArgs* a)
   a->rows = (int64_t)p.num_tokens * p.num_heads;
   split_prefix(a, num_sms);
   // The copy of the values costs about 4 bytes per value once, and saves every pair of query tiles a
-  // third of its MMA work on them.  Whole calls with and without it (8192 keys, 8 kv heads, d 128 / 64):
-  // 1 pair 56 / 41 against 55 / 39 us, 4 pairs 119 / 85 against 118 / 91, 8 pairs 201 / 152 against 209 / 164.
+  // third of its MMA work on them.  Whole calls with and without it (8192 prefix keys, 16 own keys, 32 / 8 heads),
+  // d 128: 1 pair 43 against 37 us, 2 pairs 52 / 47, 4 pairs 75 / 72, 8 pairs 109 / 110; d 64: 35 / 31, 39 / 41,
+  // 52 / 60, 83 / 102.
   const bool copy = p.act_dtype == B200_DTYPE_BFLOAT16 && p.prefix_length > 0 && a->query_pairs >= kCopyPairs;
   a->beside = p.head_size == 64 || a->query_pairs <= kBesidePairs;
   a->copy_ctas = copy ? 2 * num_sms - 1 : 0;
