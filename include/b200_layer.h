@@ -38,8 +38,10 @@ extern "C" {
  *   out_dtype T:             out = y rounded to T
  *   out_dtype FLOAT8E4M3FN:  per row (group_size 0) or per group of group_size channels (the last
  *                            group may be short): scale = max(max|y|, 1e-12) / 448 and
- *                            out = e4m3(y / scale), so out * scale stands for y.  A NaN in a
- *                            group makes its scale NaN.
+ *                            out = e4m3(y / scale), so out * scale stands for y.  Scale and
+ *                            quotient are within a few units in the last place of fp32 (products
+ *                            with reciprocals), so a y next to the middle of two codes may take
+ *                            either.  A NaN in a group makes its scale NaN.
  * out and residual_out may be x or residual themselves (each row is read before it is written).
  */
 typedef struct B200SkipRmsNormParams {

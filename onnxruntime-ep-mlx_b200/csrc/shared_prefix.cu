@@ -130,7 +130,7 @@ void launch_generic_t(const B200SharedPrefixParams& p, cudaStream_t stream) {
 // bit for magnitudes from 2^-28 to below 32 and for zero (2^11 puts that window around values of order 0.01
 // to 10); a CTA that meets any other value names its kv head, and the tensor-core pass reads that head's
 // values from the bf16 pages.  128 sequences 5 us;
-// the copy of 16384 keys of 8 heads of 128 channels 16 us (67 MB).  The tensor-core pass starts beside both.
+// the copy of 16384 keys of 8 heads of 128 channels 18 us (67 MB).  The tensor-core pass starts beside both.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 

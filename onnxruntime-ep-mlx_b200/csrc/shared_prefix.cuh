@@ -2,7 +2,8 @@
 // argument block and programmatic dependent launch.
 //
 // One call is four launches:
-//   shared_prefix_plan_kernel   lengths -> work lists (1 CTA), while the tensor-core pass starts
+//   shared_prefix_plan_kernel   lengths -> work lists (1 CTA) and, for bf16 calls of many tokens, an fp16 copy of
+//                               the prefix's values (2 CTAs per SM), while the tensor-core pass starts
 //   shared_prefix_tc_kernel     tensor-core pass (tcgen05): every token against a range of the
 //                               prefix's keys, and long chunks against their own keys
 //   shared_prefix_own_kernel    single tokens and short chunks against their own keys (memory bound)

@@ -212,7 +212,7 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 
 // x -> top * tanh(x * to_u), 32 values of a thread; the whole warp.  tanh(u) = u f(u^2) with f a polynomial of
 // degree 6, minimax in relative error over |u| <= 1 (fitted with Lawson's algorithm on 4001
-// Chebyshev-spaced points, 2000 passes; fp32 evaluation within 1.7e-7): 9 packed instructions for two
+// Chebyshev-spaced points, 2000 passes; fp32 evaluation within 1.7e-7): 10 packed instructions for two
 // values, where 1 - 2 / (1 + e^(2u)), which takes warps with a larger u, needs two MUFU operations a value.
 __device__ __forceinline__ void soft_cap(float (&x)[32], float to_u, float top) {
   float big = 0.f;
