@@ -893,6 +893,59 @@ def test_scratch_of_a_graph_ends_with_it():
         pytest.fail("scratch of deleted graphs is not freed")
 
 
+def test_scratch_of_a_graph_lives_as_long_as_it():
+    """Later eager calls, which free what ended graphs held, free nothing of a live one."""
+    call = scratch_calls()[0]
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        held = torch.cuda.memory_allocated()
+        call()
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() == held
+    del graph, outs
+
+
+def test_first_call_of_a_process_in_a_capture_is_refused():
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from onnxruntime_ep_b200 import B200Error, shared_prefix_attention
+q = torch.zeros(1, 128, device="cuda", dtype=torch.bfloat16)
+kc = torch.zeros(4, 16, 2, 64, device="cuda", dtype=torch.bfloat16)
+i = lambda *v: torch.tensor(v, device="cuda", dtype=torch.int32)
+args = (q, kc, kc.clone(), i(0, 1), i(0), i(0)[None], i(1))
+call = lambda: shared_prefix_attention(*args, prefix_length=16, num_heads=2, kv_num_heads=2, check_status=False)
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        call()
+except B200Error as e:
+    assert "cannot be captured" in str(e), e
+else:
+    raise AssertionError("captured")
+call()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = call()
+graph.replay()
+torch.cuda.synchronize()
+assert not out.any()
+del graph
+print("fine")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=os.path.join(root, "onnxruntime-ep-mlx_b200"))
+    done = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "fine", done.stderr
+
+
 def test_example_layer_against_whole_sequences():
     """The example's last decode step, recomputed from its caches with every sequence's keys in one piece."""
     import importlib.util
