@@ -20,8 +20,9 @@ if not torch.cuda.is_available():
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
 from onnxruntime_ep_b200 import (B200Error, kv_append, paged_attention, rotary_append, shared_prefix_attention,  # noqa: E402
-                                 layer, skip_rms_norm)
+                                 skip_rms_norm)
 from oracle import tolerance  # noqa: E402
+from onnxruntime_ep_b200 import layer  # noqa: E402
 
 FP8 = torch.float8_e4m3fn
 BITS = {torch.bfloat16: 8, torch.float16: 11}
